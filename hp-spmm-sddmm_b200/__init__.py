@@ -43,6 +43,10 @@ EXCHANGE_ALL_ROWS = 1
 EXCHANGE_NEEDED_ROWS_NCCL = 2
 COMM_ID_BYTES = 128
 
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
+
 VALS_ONES = 0
 VALS_U01 = 1
 VALS_UPM1 = 2
@@ -122,6 +126,17 @@ PROTOTYPES = {
     "hpspmm_layer_backward_features": (c_int, [_P, _P, _I64, _P, _P, _P]),
     "hpspmm_layer_backward_weights": (c_int, [_P, _P, _I64, _P, _P, _P, _P]),
     "hpspmm_layer_update_values": (c_int, [_P, _P, _P, _P]),
+    "hpspmm_embedding_forward": (c_int, [_P, _I64, _I64, _I64, c_int32, _P, c_int32, _P, _I64, c_float, _P, _P]),
+    "hpspmm_embedding_backward_workspace": (_I64, [_I64, _I64, _I64]),
+    "hpspmm_embedding_backward": (c_int, [_P, _I64, _I64, _I64, c_int32, _P, c_int32, _P, _I64, c_float, _P, _P,
+                                          c_size_t, _P]),
+    "hpspmm_grouped_product": (c_int, [_P, _I64, _I64, _I64, _I64, c_int32, _P, _I64, _P, c_int32, _P, _P, _P]),
+    "hpspmm_grouped_weight_grad": (c_int, [_P, _I64, _I64, _I64, _I64, c_int32, _P, _I64, _P, _I64, _P, _P, c_int32,
+                                           _P]),
+    "hpspmm_topk_distill_forward": (c_int, [_P, _I64, _I64, _I64, c_int32, _P, _I64, _P, c_int32, _P, c_float, _P, _P,
+                                            _P]),
+    "hpspmm_topk_distill_backward": (c_int, [_P, _I64, _I64, _I64, c_int32, _P, _I64, _P, c_int32, _P, c_float, _P, _P,
+                                             _I64, _P, _P]),
     "hpspmm_padded_nnz": (_I64, [_I64, _I64]),
     "hpspmm_csr_to_coo_padded": (c_int, [_P, _I64, _I64, _P, _P, _P, _I64, _P, _P, _P, _P]),
     "hpspmm_csr_to_coo_reordered": (c_int, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _P]),
@@ -446,6 +461,40 @@ class Context:
         st = self.lib.hpspmm_validate_csr(self.handle, M, N, nnz, _ptr(row_ptr), _ptr(col_idx),
                                           byref(bad), stream)
         return st, bad.value
+
+    # -- dense operands by index ----------------------------------------------------
+    def embedding_forward(self, T, N, K, dtype, ids, id_bytes, table, ld_table, scale, out, stream=None):
+        self._check(self.lib.hpspmm_embedding_forward(self.handle, T, N, K, dtype, _ptr(ids), id_bytes, _ptr(table),
+                                                      ld_table, scale, _ptr(out), stream), "hpspmm_embedding_forward")
+
+    def embedding_backward(self, T, N, K, dtype, ids, id_bytes, dout, ld_dout, scale, dtable, workspace,
+                           workspace_bytes, stream=None):
+        self._check(self.lib.hpspmm_embedding_backward(self.handle, T, N, K, dtype, _ptr(ids), id_bytes, _ptr(dout),
+                                                       ld_dout, scale, _ptr(dtable), _ptr(workspace), workspace_bytes,
+                                                       stream), "hpspmm_embedding_backward")
+
+    def grouped_product(self, R, G, K, N, dtype, X, ldx, W, w_out_first, offsets, Y, stream=None):
+        self._check(self.lib.hpspmm_grouped_product(self.handle, R, G, K, N, dtype, _ptr(X), ldx, _ptr(W),
+                                                    int(w_out_first), _ptr(offsets), _ptr(Y), stream),
+                    "hpspmm_grouped_product")
+
+    def grouped_weight_grad(self, R, G, K, N, dtype, X, ldx, dY, ldy, offsets, dW, w_out_first, stream=None):
+        self._check(self.lib.hpspmm_grouped_weight_grad(self.handle, R, G, K, N, dtype, _ptr(X), ldx, _ptr(dY), ldy,
+                                                        _ptr(offsets), _ptr(dW), int(w_out_first), stream),
+                    "hpspmm_grouped_weight_grad")
+
+    def topk_distill_forward(self, T, V, k, dtype, logits, ld, ids, id_bytes, teacher, temperature, loss, stats=None,
+                             stream=None):
+        self._check(self.lib.hpspmm_topk_distill_forward(self.handle, T, V, k, dtype, _ptr(logits), ld, _ptr(ids),
+                                                         id_bytes, _ptr(teacher), temperature, _ptr(loss), _ptr(stats),
+                                                         stream), "hpspmm_topk_distill_forward")
+
+    def topk_distill_backward(self, T, V, k, dtype, logits, ld, ids, id_bytes, teacher, temperature, stats, dloss,
+                              dloss_stride, dlogits, stream=None):
+        self._check(self.lib.hpspmm_topk_distill_backward(self.handle, T, V, k, dtype, _ptr(logits), ld, _ptr(ids),
+                                                          id_bytes, _ptr(teacher), temperature, _ptr(stats),
+                                                          _ptr(dloss), dloss_stride, _ptr(dlogits), stream),
+                    "hpspmm_topk_distill_backward")
 
     def launch_count(self):
         return self.lib.hpspmm_ctx_launch_count(self.handle)

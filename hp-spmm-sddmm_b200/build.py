@@ -31,6 +31,9 @@ SOURCES = [
     "coo_kernels.cu",
     "sddmm_kernels.cu",
     "layer_grad_kernels.cu",
+    "embedding_kernels.cu",
+    "grouped_kernels.cu",
+    "distill_kernels.cu",
     "structure_kernels.cu",
     "graph_layer.cu",
     "probe_kernels.cu",
@@ -104,15 +107,15 @@ def _stale(out, *sources):
 
 
 def build_bindings(force=False, verbose=False):
-    """Builds the CPython extensions: the hot calls of the C ABI, and the PyTorch operators of the layer."""
+    """Builds the CPython extensions: the hot calls of the C ABI, and the PyTorch operators."""
     build(force=force, verbose=verbose)
     python_inc = ["-I", sysconfig.get_paths()["include"], "-I", os.path.join(ROOT, "include")]
     common = [_cxx(), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
     src = os.path.join(CSRC, "python_binding.cpp")
     if force or _stale(NATIVE_PATH, src):
         _run(common + python_inc + [src, "-o", NATIVE_PATH], verbose)
-    src = os.path.join(CSRC, "torch_binding.cpp")
-    if force or _stale(TORCH_PATH, src):
+    srcs = [os.path.join(CSRC, f) for f in ("torch_binding.cpp", "torch_dense_binding.cpp")]
+    if force or _stale(TORCH_PATH, *srcs):
         import torch
         t = os.path.dirname(torch.__file__)
         inc = []
@@ -121,7 +124,7 @@ def build_bindings(force=False, verbose=False):
             inc += ["-isystem", d]
         _run(common + python_inc + inc +
              ["-DTORCH_EXTENSION_NAME=_hpspmm_torch", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi()),
-              src, "-o", TORCH_PATH, "-L", LIB_DIR, "-lhpspmm", "-L", os.path.join(t, "lib"), "-lc10", "-lc10_cuda",
+              *srcs, "-o", TORCH_PATH, "-L", LIB_DIR, "-lhpspmm", "-L", os.path.join(t, "lib"), "-lc10", "-lc10_cuda",
               "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], verbose)
     return NATIVE_PATH, TORCH_PATH
 

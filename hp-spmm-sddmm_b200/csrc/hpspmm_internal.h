@@ -176,6 +176,11 @@ static inline int hpspmm_set_err(hpspmm_ctx* ctx, int status, const char* what, 
     }                                                                      \
   } while (0)
 
+static inline int hpspmm_unsupported(hpspmm_ctx* ctx, const char* what) {
+  if (ctx) snprintf(ctx->err, sizeof(ctx->err), "unsupported: %s", what);
+  return HPSPMM_ERR_UNSUPPORTED;
+}
+
 // Makes the context's device current for the calling thread for the duration of a call.
 struct hpspmm_device_guard {
   int prev;

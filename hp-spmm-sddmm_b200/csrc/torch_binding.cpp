@@ -288,7 +288,10 @@ void forget_layer(int64_t id) {
 
 }  // namespace
 
+void bind_dense_operators(py::module_& m);   // torch_dense_binding.cpp
+
 PYBIND11_MODULE(_hpspmm_torch, m) {
+  bind_dense_operators(m);
   m.def("register_layer", &register_layer);
   m.def("forget_layer", &forget_layer, py::call_guard<py::gil_scoped_release>());
   m.def("layer_forward", [](const Tensor& H, const Tensor& vals, int64_t id) { return op_forward().call(H, vals, id); },

@@ -1,13 +1,18 @@
-"""PyTorch front-end of the aggregation layer: autograd over the C ABI, no PyTorch arithmetic.
+"""PyTorch front-end of the aggregation layer and of what stands beside it: autograd over the C ABI, no PyTorch arithmetic.
 
     layer = TorchLayer(row_ptr, col_idx, vals, M, N, max_K)   # CUDA tensors, int32 / int32 / float32
     C = layer(H)                                              # C = A·H, differentiable in H and in vals
     C.sum().backward()                                        # dH = Aᵀ·dC (SpMM), dvals = SDDMM(dC, H)
 
-Four operators are registered under the namespace ``hpspmm`` (``layer_forward``,
+    E = embedding(ids, table, scale)                          # rows of a table by id, differentiable in the table
+    Y = grouped_product(X, W, offsets)                        # one matrix for each group of rows, differentiable in X and W
+    loss = topk_distill_loss(logits, teacher_ids, teacher_logits, temperature)   # one value a row
+
+For the layer four operators are registered under the namespace ``hpspmm`` (``layer_forward``,
 ``layer_backward_features``, ``layer_backward_weights``, and ``layer_backward`` for both gradients at
 once) by csrc/torch_binding.cpp, with an autograd formula that chains them; the shape functions for tracing are below, so the layer can sit inside a
-compiled or exported module.  Every operator calls ``hpspmm_layer_*`` of libhpspmm.so on the current
+compiled or exported module.  The three functions have six more (csrc/torch_dense_binding.cpp): ``embedding``,
+``grouped_product`` and ``topk_distill`` with their gradients.  Every operator calls libhpspmm.so on the current
 CUDA stream of the input's device; a CPU tensor is rejected (there is no fallback).  PyTorch supplies
 memory, streams and the autograd tape only.
 
@@ -109,3 +114,76 @@ class TorchLayer:
             self.close()
         except Exception:
             pass
+
+
+# ---- dense operands by index -----------------------------------------------------------------------------------
+
+def _plain(*tensors):
+    """Whether a call may skip the Python dispatcher: tracers, tensor subclasses and function modes have to see it."""
+    return not (torch.compiler.is_compiling() or not all(isinstance(t, torch.Tensor) for t in tensors)
+                or has_torch_function_variadic(*tensors))
+
+
+@torch.library.register_fake("hpspmm::embedding")
+def _(ids, table, scale):
+    return table.new_empty((*ids.shape, table.shape[1]))
+
+
+@torch.library.register_fake("hpspmm::embedding_backward")
+def _(grad, ids, rows, scale):
+    return grad.new_empty((rows, grad.shape[-1]))
+
+
+@torch.library.register_fake("hpspmm::grouped_product")
+def _(X, W, offsets):
+    return X.new_empty((X.shape[0], W.shape[2]))
+
+
+@torch.library.register_fake("hpspmm::grouped_weight_grad")
+def _(X, dY, offsets, transposed):
+    G, K, N = offsets.shape[0] - 1, X.shape[1], dY.shape[1]
+    return X.new_empty((G, N, K)).transpose(1, 2) if transposed else X.new_empty((G, K, N))
+
+
+@torch.library.register_fake("hpspmm::topk_distill")
+def _(logits, teacher_ids, teacher_logits, temperature):
+    loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+    return loss, loss.new_empty((loss.numel(), 2))
+
+
+@torch.library.register_fake("hpspmm::topk_distill_backward")
+def _(dloss, logits, teacher_ids, teacher_logits, stats, temperature):
+    return logits.new_empty(logits.shape)
+
+
+def embedding(ids, table, scale=1.0):
+    """``scale * table[ids]``: ids int32 or int64 of any shape, table [N, K] in float32, float16 or bfloat16.
+
+    An id outside [0, N) (the -1 of a padded batch) gives a row of zeros and takes no part in the gradient.  The
+    gradient of the table is dense, summed in 32 bits in an order that does not change from call to call.  A routed
+    layer's rows by slot are such a lookup too, and their gradient such a sum."""
+    if _plain(ids, table):
+        return _C.embedding(ids, table, scale)
+    return torch.ops.hpspmm.embedding.default(ids, table, scale)
+
+
+def grouped_product(X, W, offsets):
+    """``Y[r] = X[r] @ W[g]`` for the rows offsets[g] <= r < offsets[g + 1]: X [R, K], W [G, K, N], offsets [G + 1]
+    ascending int32 on the GPU.  Rows of no group (behind the last one of a padded batch) become zeros.
+
+    W may be the transpose of a contiguous [G, N, K] (``W.transpose(1, 2)`` of the weights of linear layers): it is
+    read as it lies, and its gradient lies the same way.  float32, float16 or bfloat16, all of one type."""
+    if _plain(X, W, offsets):
+        return _C.grouped_product(X, W, offsets)
+    return torch.ops.hpspmm.grouped_product.default(X, W, offsets)
+
+
+def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0):
+    """``temperature**2 * KL(teacher || student)`` of every row, the teacher known by its k largest logits: logits
+    [..., V], teacher_ids (int32 or int64) and teacher_logits [..., k], k up to 1024; float32 [...] comes out.
+
+    The teacher's softmax runs over the entries whose id lies in [0, V) and whose logit is above -inf; a row without
+    any has loss 0 and a gradient of zeros.  Differentiable in the logits, once."""
+    if _plain(logits, teacher_ids, teacher_logits):
+        return _C.topk_distill(logits, teacher_ids, teacher_logits, temperature)
+    return torch.ops.hpspmm.topk_distill.default(logits, teacher_ids, teacher_logits, temperature)[0]

@@ -320,6 +320,66 @@ HPSPMM_API int hpspmm_layer_backward(hpspmm_ctx* ctx, hpspmm_layer* layer, int64
 HPSPMM_API int hpspmm_layer_update_values(hpspmm_ctx* ctx, hpspmm_layer* layer,
                                           const float* vals, hpspmm_stream stream);
 
+/* ---- dense operands by index: tables, groups of rows, teachers ------------------------------------------
+ * Operators next to the sparse products whose pattern is so regular that no CSR of it is built: one entry to a row
+ * (rows of a table by id), one block to a group of rows (a matrix for each relation type or expert), a few samples to a
+ * row (a teacher's largest logits).  Element types below; sums are kept in 32 bits and rounded once.  Rows of the
+ * operands that are read may lie `ld` elements apart, what is written is contiguous.  All of them only enqueue
+ * kernels: no allocation, no synchronisation, no state between calls, so they can be captured into a CUDA graph, and
+ * calls that share a context may overlap on the GPU (not on the host: one call on a context at a time).  The
+ * reference has no counterpart. */
+enum { HPSPMM_TYPE_F32 = 0, HPSPMM_TYPE_F16 = 1, HPSPMM_TYPE_BF16 = 2 };
+
+/* out[t, :] = scale * table[ids[t], :]    table N x K, out T x K; ids of id_bytes (4 or 8) bytes.  An id outside
+ * [0, N), such as the -1 of a padded batch, is a row without an entry: zeros. */
+HPSPMM_API int hpspmm_embedding_forward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, int32_t type,
+                                        const void* ids, int32_t id_bytes, const void* table,
+                                        int64_t ld_table, float scale, void* out,
+                                        hpspmm_stream stream);
+/* dTable[v, :] = scale * sum of dOut[t, :] over the t with ids[t] = v, zeros for rows no id names.  Deterministic:
+ * positions are sorted by id and added in an order that depends on the sizes and the ids alone.  workspace: device
+ * memory of hpspmm_embedding_backward_workspace bytes (-1: a size is negative or above 2^31 - 2), aligned to 256
+ * bytes, that no other call uses until this one is done; it needs no initial value. */
+HPSPMM_API int64_t hpspmm_embedding_backward_workspace(int64_t T, int64_t N, int64_t K);
+HPSPMM_API int hpspmm_embedding_backward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, int32_t type,
+                                         const void* ids, int32_t id_bytes, const void* dOut,
+                                         int64_t ld_dout, float scale, void* dTable, void* workspace,
+                                         size_t workspace_bytes, hpspmm_stream stream);
+
+/* Y[r, :] = X[r, :] * W[g] for the rows offsets[g] <= r < offsets[g + 1] of group g: X R x K, Y R x N, W G matrices
+ * K x N one after the other (w_out_first = 0) or stored transposed, N x K (w_out_first = 1), offsets G + 1 ascending
+ * device ints in [0, R].  Rows in front of the first group and behind the last one become zeros.  The gradient of X is
+ * the same call with dY, K and N exchanged and the other w_out_first.  Offsets that do not ascend give rows of no use,
+ * but nothing outside the operands is read or written. */
+HPSPMM_API int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N,
+                                      int32_t type, const void* X, int64_t ldx, const void* W,
+                                      int32_t w_out_first, const int32_t* offsets, void* Y,
+                                      hpspmm_stream stream);
+/* dW[g] = X_g^T * dY_g over the rows of group g, stored as w_out_first says; zeros for a group without rows. */
+HPSPMM_API int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N,
+                                          int32_t type, const void* X, int64_t ldx, const void* dY,
+                                          int64_t ldy, const int32_t* offsets, void* dW,
+                                          int32_t w_out_first, hpspmm_stream stream);
+
+/* For every row z of T x V logits and the k entries (ids[j], teacher_logits[j]) its teacher kept:
+ *   p    = softmax over the entries of teacher_logits / temperature
+ *   loss = temperature^2 * sum_j p_j (log p_j - log softmax(z / temperature)[ids[j]])
+ * An entry counts when its id lies in [0, V) and its logit is above -infinity; ids that come twice count twice.  A row
+ * without entries has loss 0.  k is at most 1024 (HPSPMM_ERR_UNSUPPORTED beyond).  loss: T floats.  stats: T x 2
+ * floats for the gradient (largest logit of the row, sum of exp((z - it) / temperature)), or NULL. */
+HPSPMM_API int hpspmm_topk_distill_forward(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int32_t type,
+                                           const void* logits, int64_t ld_logits, const void* ids,
+                                           int32_t id_bytes, const float* teacher_logits,
+                                           float temperature, float* loss, float* stats,
+                                           hpspmm_stream stream);
+/* dlogits[t, v] = dloss[t] * temperature * (softmax(z / temperature)_v - sum of p_j over the entries j with id v);
+ * zeros for a row without entries.  dloss: T floats dloss_stride apart (0: the same for all rows). */
+HPSPMM_API int hpspmm_topk_distill_backward(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int32_t type,
+                                            const void* logits, int64_t ld_logits, const void* ids,
+                                            int32_t id_bytes, const float* teacher_logits,
+                                            float temperature, const float* stats, const float* dloss,
+                                            int64_t dloss_stride, void* dlogits, hpspmm_stream stream);
+
 /* ---- CSR -> padded COO (device) ------------------------------------------------------
  * Replaces the host loops of get_coo_mat_from_smtx (spmm/mm/spmm_common.cpp:210-226):
  * row_out[j] = row of entry j, then (0, 0, 0.0f) padding up to a multiple of `padding`.

@@ -1,0 +1,43 @@
+"""What the dense operators by index say without a GPU: CPU tensors and bad arguments are refused, shapes are known."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import dense_reference as ref  # noqa: E402
+
+
+def test_cpu_tensors_are_refused(pkg):
+    ops = ref.ops_of(pkg)
+    ids, x = torch.zeros(3, dtype=torch.int64), torch.zeros((3, 4))
+    off = torch.zeros(2, dtype=torch.int32)
+    calls = [lambda: ops.embedding(ids, x), lambda: torch.ops.hpspmm.embedding_backward(x, ids, 5, 1.0),
+             lambda: ops.grouped_product(x, torch.zeros((1, 4, 2)), off),
+             lambda: torch.ops.hpspmm.grouped_weight_grad(x, x, off, False),
+             lambda: ops.topk_distill_loss(x, torch.zeros((3, 2), dtype=torch.int64), torch.zeros((3, 2))),
+             lambda: torch.ops.hpspmm.topk_distill_backward(x[:, 0], x, torch.zeros((3, 2), dtype=torch.int64),
+                                                            torch.zeros((3, 2)), torch.zeros((3, 2)), 1.0)]
+    for f in calls:
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            f()
+
+
+def test_null_contexts_are_refused(pkg):
+    lib = pkg.load_library()
+    i64 = ctypes.c_int64
+    for name in ("embedding_forward", "embedding_backward", "grouped_product", "grouped_weight_grad", "topk_distill_forward",
+                 "topk_distill_backward"):
+        args = [0 if t in (i64, ctypes.c_int32, ctypes.c_size_t) else 1.0 if t is ctypes.c_float else None
+                for t in pkg.PROTOTYPES["hpspmm_" + name][1]]
+        assert getattr(lib, "hpspmm_" + name)(*args) == pkg.ERR_INVALID
+
+
+def test_workspace_sizes(pkg):
+    need = pkg.load_library().hpspmm_embedding_backward_workspace
+    assert need(0, 5, 5) >= 0 and need(-1, 5, 5) == -1 and need(5, -1, 5) == -1 and need(5, 5, -1) == -1
+    assert need(1 << 31, 5, 5) == -1 and need(5, 1 << 31, 5) == -1
+    last = 0
+    for T in (1, 100, 8192, 8193, 1 << 20, 1 << 26):      # grows with the batch, stays far below the operands
+        got = need(T, 100_000, 64)
+        assert got >= 8 * T and got >= last
+        last = got

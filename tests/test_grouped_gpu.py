@@ -1,0 +1,270 @@
+"""One matrix for each group of rows: the product and its gradients (needs a B200)."""
+import pytest
+
+torch = pytest.importorskip("torch")
+import dense_reference as ref  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    return ref.ops_of(pkg)
+
+
+def _offsets(sizes, first=0):
+    return torch.tensor([first] + sizes, device="cuda").cumsum(0).int()
+
+
+def _weights(G, K, N, dtype, gen, transposed):
+    w = torch.randn((G, N, K) if transposed else (G, K, N), device="cuda", generator=gen).to(dtype)
+    return w.transpose(1, 2) if transposed else w
+
+
+def _check(ops, X, W, offsets, dY):
+    x, w = X.detach().requires_grad_(), W.detach().requires_grad_()
+    y = ops.grouped_product(x, w, offsets)
+    want, tol = ref.grouped(X, W, offsets)
+    assert y.shape == want.shape and y.dtype == X.dtype and ref.outside(y.detach(), want, tol) == 0
+    dx, dw = torch.autograd.grad(y, (x, w), dY)
+    want, tol = ref.grouped(dY, W.transpose(1, 2), offsets)
+    assert dx.shape == X.shape and ref.outside(dx, want, tol) == 0
+    want, tol = ref.grouped_weight(X, dY, offsets)
+    assert dw.shape == W.shape and dw.dtype == X.dtype and ref.outside(dw, want, tol) == 0
+    return y, dx, dw
+
+
+SIZES = [([1], 1, 1), ([0], 8, 8), ([5], 3, 2), ([64], 64, 64), ([1], 2048, 128), ([3, 0, 1, 2], 256, 512), ([17, 300, 0, 64, 1], 72, 136),
+         ([129, 127, 128, 257], 64, 256), ([33] * 40, 40, 24), ([1000, 1], 264, 520), ([0, 0, 700, 0], 100, 64),
+         ([63, 65, 191], 333, 131), ([2] * 70, 128, 384), ([515], 1000, 8), ([16, 48, 240, 272, 496], 320, 320)]
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("sizes,K,N", SIZES)
+def test_sizes_and_types(ops, type, transposed, sizes, K, N):
+    gen = torch.Generator("cuda").manual_seed(K + N + len(sizes))
+    R = sum(sizes)
+    X = torch.randn((R, K), device="cuda", generator=gen).to(ref.TYPES[type])
+    dY = torch.randn((R, N), device="cuda", generator=gen).to(ref.TYPES[type])
+    _check(ops, X, _weights(len(sizes), K, N, X.dtype, gen, transposed), _offsets(sizes), dY)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("K,N", [(128, 192), (50, 30)])
+@pytest.mark.parametrize("first,behind", [(0, 9), (5, 0), (70, 200), (0, 0)])
+def test_rows_of_no_group(ops, type, K, N, first, behind):
+    """Rows in front of the first group and behind the last one: zeros in Y and dX, nothing in dW, whatever they hold."""
+    gen = torch.Generator("cuda").manual_seed(first + behind)
+    sizes = [40, 0, 130, 7]
+    R = first + sum(sizes) + behind
+    X = torch.randn((R, K), device="cuda", generator=gen).to(ref.TYPES[type])
+    dY = torch.randn((R, N), device="cuda", generator=gen).to(ref.TYPES[type])
+    X[:first], dY[:first] = float("nan"), float("inf")
+    X[first + sum(sizes):], dY[first + sum(sizes):] = float("inf"), float("nan")
+    W = _weights(4, K, N, X.dtype, gen, False)
+    y, dx, dw = _check(ops, X, W, _offsets(sizes, first), dY)
+    for t in (y, dx):
+        assert not t[:first].any() and not t[first + sum(sizes):].any()
+    assert not dw[1].any()
+
+
+@pytest.mark.parametrize("K,N", [(128, 256), (36, 20)])
+def test_infinities_stay_in_their_rows_and_groups(ops, K, N):
+    gen = torch.Generator("cuda").manual_seed(K)
+    sizes = [20, 30, 50, 70]
+    for dtype in (torch.bfloat16, torch.float32):
+        X, dY = (torch.randn((170, c), device="cuda", generator=gen).to(dtype) for c in (K, N))
+        W = _weights(4, K, N, dtype, gen, False)
+        X[20, 3], X[49, 0], W[3, 0, 0], dY[100, N - 1] = float("nan"), float("inf"), float("inf"), float("nan")
+        y = ops.grouped_product(X, W, _offsets(sizes))
+        dx = ops.grouped_product(dY, W.transpose(1, 2), _offsets(sizes))
+        dw = torch.ops.hpspmm.grouped_weight_grad(X, dY, _offsets(sizes), False)
+        rows = torch.ones(170, dtype=torch.bool, device="cuda")
+        rows[[20, 49]] = False
+        rows[100:] = False
+        want, tol = ref.grouped(X, W, _offsets(sizes))
+        assert ref.outside(y[rows], want[rows], tol[rows]) == 0
+        assert bool(torch.isnan(y[20]).all()) and not torch.isfinite(y[49]).any()
+        want, tol = ref.grouped(dY[:100], W.transpose(1, 2), _offsets([20, 30, 50, 0]))
+        assert ref.outside(dx[:100], want, tol) == 0 and bool(torch.isnan(dx[100]).all())
+        want, tol = ref.grouped_weight(X, dY, _offsets(sizes))
+        for g in (0, 2):                              # groups whose neighbours hold what spreads
+            assert ref.outside(dw[g], want[g], tol[g]) == 0
+        assert torch.equal(torch.isnan(dw[3]), torch.isnan(want[3]))
+
+
+def test_many_groups_and_none(ops):
+    gen = torch.Generator("cuda").manual_seed(1)
+    sizes = torch.randint(0, 5, (3001,), generator=torch.Generator().manual_seed(2)).tolist()
+    for K, N in ((64, 64), (24, 40), (7, 5)):
+        for dtype in (torch.float16, torch.float32):
+            X, dY = (torch.randn((sum(sizes), c), device="cuda", generator=gen).to(dtype) for c in (K, N))
+            _check(ops, X, _weights(3001, K, N, dtype, gen, True), _offsets(sizes), dY)
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    X = torch.randn((5, 64), device="cuda", generator=gen)
+    assert not ops.grouped_product(X, X.new_empty((0, 64, 16)), none).any()
+    assert torch.ops.hpspmm.grouped_weight_grad(X, X, none, False).shape == (0, 64, 64)
+    for K, N in ((0, 16), (16, 0)):
+        y = ops.grouped_product(X[:, :K], X.new_empty((1, K, N)), _offsets([5]))
+        assert y.shape == (5, N) and not y.any()
+        assert torch.ops.hpspmm.grouped_weight_grad(X[:, :K], y, _offsets([5]), True).shape == (1, K, N)
+    assert ops.grouped_product(X[:0], X.new_empty((2, 64, 16)), _offsets([0, 0])).shape == (0, 16)
+    assert not torch.ops.hpspmm.grouped_weight_grad(X[:0], X[:0], _offsets([0, 0]), False).any()
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_strides(ops, type):
+    gen = torch.Generator("cuda").manual_seed(4)
+    sizes, dtype = [100, 30, 66], ref.TYPES[type]
+    big = torch.randn((400, 320), device="cuda", generator=gen).to(dtype)
+    W = _weights(3, 128, 64, dtype, gen, False)
+    dys = big[200:396, 100:164], big[4:200, :64], big[:196, 1:65], big[:1, :64].expand(196, 64), big[:196, :1].expand(196, 64)
+    for X, dY in zip((big[:196, :128], big[:196, 8:136], big[:196, 3:131], big[::2][:196, :128], big.T[:196, 64:192]), dys):
+        _check(ops, X, W, _offsets(sizes), dY)
+    X, dY = big[:196, :128], big[:196, 128:192]
+    for w in (W[:, :, ::2].repeat_interleave(2, 2)[:, :, :64], W[:1].expand(3, 128, 64), W.transpose(0, 1).contiguous().transpose(0, 1)):
+        _check(ops, X, w, _offsets(sizes), dY)
+    spaced = torch.stack([_offsets(sizes), _offsets(sizes)], 1)[:, 0]
+    assert torch.equal(ops.grouped_product(X, W, spaced), ops.grouped_product(X, W, _offsets(sizes)))
+    # memory that begins 2 or 4 bytes off a 16-byte boundary
+    flat = torch.randn(3 * 128 * 64 + 1, device="cuda", generator=gen).to(dtype)
+    _check(ops, X, flat[1:].view(3, 128, 64), _offsets(sizes), dY)
+    # one matrix for all groups, from a smaller leaf: its gradient is the sum over the groups
+    leaf = W[:1].clone().requires_grad_()
+    ops.grouped_product(X, leaf.expand(3, 128, 64), _offsets(sizes)).backward(dY)
+    parts, tol = ref.grouped_weight(X, dY, _offsets(sizes))
+    want = parts.sum(0, keepdim=True)
+    assert ref.outside(leaf.grad, want, tol.sum(0, keepdim=True) + 3 * ref.rounding(dtype, parts.abs().sum(0, keepdim=True))) == 0
+
+
+def test_offsets_that_do_not_ascend_stay_in_bounds(ops):
+    """The values are of no use, but nothing outside the operands is touched and rows that are named once are right."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    for dtype in (torch.bfloat16, torch.float32):
+        for K, N in ((128, 64), (33, 20)):
+            X, dY = (torch.randn((90, c), device="cuda", generator=gen).to(dtype) for c in (K, N))
+            W = _weights(3, K, N, dtype, gen, False)
+            for bad in ([-5, 30, 1000, 2 ** 31 - 1], [0, 60, 20, 90], [90, 60, 30, 0], [2 ** 31 - 1, -2 ** 31, 0, 7]):
+                off = torch.tensor(bad, dtype=torch.int32, device="cuda")
+                y = ops.grouped_product(X, W, off)
+                dw = torch.ops.hpspmm.grouped_weight_grad(X, dY, off, False)
+                assert y.shape == (90, N) and dw.shape == (3, K, N)
+            off = torch.tensor([-5, 30, 1000, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+            want, tol = ref.grouped(X, W, _offsets([30, 60, 0]))
+            assert ref.outside(ops.grouped_product(X, W, off), want, tol) == 0
+
+
+def test_same_every_time_captured_and_on_another_stream(ops):
+    gen = torch.Generator("cuda").manual_seed(6)
+    side = torch.cuda.Stream()
+    for dtype, sizes, K, N in ((torch.bfloat16, [3, 0, 1, 9], 1024, 256), (torch.bfloat16, [300, 40, 500, 7], 256, 384),
+                               (torch.float32, [100, 0, 31, 7], 60, 36)):
+        R = sum(sizes) + 5
+        X, dY = (torch.randn((R, c), device="cuda", generator=gen).to(dtype) for c in (K, N))
+        W, off = _weights(4, K, N, dtype, gen, False), _offsets(sizes)
+
+        def step():
+            return (ops.grouped_product(X, W, off), ops.grouped_product(dY, W.transpose(1, 2), off),
+                    torch.ops.hpspmm.grouped_weight_grad(X, dY, off, False))
+
+        first = step()
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(first, step()))
+        side.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            held = step()
+        X.mul_(2), off.copy_(_offsets(sizes[::-1]))
+        torch.cuda.synchronize()
+        g.replay()
+        with torch.cuda.stream(side):
+            eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager))
+        want, tol = ref.grouped(X, W, off)
+        assert ref.outside(held[0], want, tol) == 0
+
+
+def test_gradients_against_differences_and_second_derivatives(ops):
+    gen = torch.Generator("cuda").manual_seed(7)
+    sizes = [10, 0, 25]
+    X, dY = (torch.randn((35, c), device="cuda", generator=gen).requires_grad_() for c in (20, 12))
+    W = _weights(3, 20, 12, torch.float32, gen, False).requires_grad_()
+    off = _offsets(sizes)
+    ways = [torch.randn_like(X), torch.randn_like(W)]
+    dx, dw = torch.autograd.grad(ops.grouped_product(X, W, off), (X, W), dY, create_graph=True)
+    with torch.no_grad():
+        for leaf, way, got in ((X, ways[0], dx), (W, ways[1], dw)):
+            def f(t):
+                return (ops.grouped_product(*((t, W) if leaf is X else (X, t)), off).double() * dY.double()).sum()
+            # linear in each operand: exact but for the roundings of 35 x 12 sums of 20 products
+            assert abs(float((f(leaf + way) - f(leaf - way)) / 2 - (got.double() * way.double()).sum())) < 35 * 12 * 20 * 2.0 ** -20
+    # derivatives of the gradients, each along a random way
+    a, b = (t.detach().double().requires_grad_() for t in (X, W))
+    d = dY.detach().double().requires_grad_()
+    y = torch.cat([a[s:e] @ b[g] for g, (s, e) in enumerate(zip(off.tolist(), off.tolist()[1:]))])
+    ra, rb = torch.autograd.grad(y, (a, b), d, create_graph=True)
+    for got, want, way in ((dx, ra, ways[0]), (dw, rb, ways[1])):
+        g = torch.autograd.grad(got, (X, W, dY), way, retain_graph=True, allow_unused=True)
+        w = torch.autograd.grad(want, (a, b, d), way.double(), retain_graph=True, allow_unused=True)
+        for p, q in zip(g, w):
+            assert (p is None) == (q is None)
+            if q is not None:
+                assert ref.outside(p, q, torch.full_like(q, 40 * 2.0 ** -23 * 40 * 16)) == 0     # 35 products of values below 4
+
+
+def test_more_than_2_31_elements(ops):
+    # weights: group 519 lies behind 2^31 elements
+    G, K, N = 520, 2048, 2056
+    W = torch.zeros((G, K, N), dtype=torch.bfloat16, device="cuda")
+    W[-1] = torch.randn((K, N), device="cuda") / 45
+    X = torch.randn((3, K), device="cuda").bfloat16()
+    off = _offsets([1] + [0] * (G - 2) + [2])
+    want, tol = ref.grouped(X[1:], W[-1:], _offsets([2]))
+    y = ops.grouped_product(X, W, off)
+    assert ref.outside(y[1:], want, tol) == 0 and not y[0].any()
+    dw = torch.ops.hpspmm.grouped_weight_grad(X, y, off, False)
+    want, tol = ref.grouped_weight(X[1:], y[1:], _offsets([2]))
+    assert ref.outside(dw[-1:], want, tol) == 0 and not dw[:-1].any()
+    del W, dw
+    for K, dtype in ((2056, torch.bfloat16), (515, torch.float32)):        # rows
+        R = (2 ** 31 + 5_000_000) // K
+        X = torch.zeros((R, K), dtype=dtype, device="cuda")
+        X[-70:] = torch.randn((70, K), device="cuda")
+        W = _weights(2, K, 16, dtype, None, False)
+        off = torch.tensor([0, R - 66, R], dtype=torch.int32, device="cuda")
+        y = ops.grouped_product(X, W, off)
+        want, tol = ref.grouped(X[-70:], W, _offsets([4, 66]))
+        assert ref.outside(y[-70:], want, tol) == 0
+        dx = ops.grouped_product(y, W.transpose(1, 2), off)
+        want, tol = ref.grouped(y[-70:], W.transpose(1, 2), _offsets([4, 66]))
+        assert ref.outside(dx[-70:], want, tol) == 0
+        dw = torch.ops.hpspmm.grouped_weight_grad(X, y, off, True)
+        want, tol = ref.grouped_weight(X[-70:], y[-70:], _offsets([4, 66]))
+        assert ref.outside(dw[1], want[1], tol[1]) == 0
+        del X, y, dx
+
+
+def test_refusals(ops, pkg, gpu_ctx):
+    X, W, off = torch.zeros((6, 8), device="cuda"), torch.zeros((2, 8, 4), device="cuda"), _offsets([3, 3])
+    ops.grouped_product(X, W, off)
+    for args in ((X.double(), W.double(), off), (X.half(), W, off), (X, W[0], off), (X[:, :7], W, off), (X, W, off.long()),
+                 (X, W, off[:2]), (X, W, off.cpu()), (X.cpu(), W.cpu(), off.cpu()), (X, W.cpu(), off), (X[0], W, off)):
+        with pytest.raises(RuntimeError, match="hpspmm"):
+            ops.grouped_product(*args)
+    grad = torch.ops.hpspmm.grouped_weight_grad
+    for args in ((X, X[:5], off), (X, X.half(), off), (X, X, off.long()), (X, X, off[:0]), (X, X[0], off), (X, X, off[None])):
+        with pytest.raises(RuntimeError, match="hpspmm"):
+            grad(*args, False)
+    Y = torch.zeros((6, 4), device="cuda")
+    good = [6, 2, 8, 4, pkg.TYPE_F32, X.data_ptr(), 8, W.data_ptr(), 0, off.data_ptr(), Y.data_ptr()]
+    gpu_ctx.grouped_product(*good)
+    for at, v in ((0, -1), (1, -1), (2, -1), (3, -1), (4, 7), (5, None), (6, -1), (7, None), (9, None), (10, None), (0, 1 << 31)):
+        with pytest.raises(pkg.HpspmmError):
+            gpu_ctx.grouped_product(*(good[:at] + [v] + good[at + 1:]))
+    good = [6, 2, 8, 4, pkg.TYPE_F32, X.data_ptr(), 8, Y.data_ptr(), 4, off.data_ptr(), W.data_ptr(), 0]
+    gpu_ctx.grouped_weight_grad(*good)
+    for at, v in ((0, -1), (4, -1), (5, None), (6, -1), (7, None), (8, -1), (9, None), (10, None), (1, 1 << 40)):
+        with pytest.raises(pkg.HpspmmError):
+            gpu_ctx.grouped_weight_grad(*(good[:at] + [v] + good[at + 1:]))
