@@ -176,6 +176,7 @@ PROTOTYPES = {
     "hpspmm_probe_gather_gbs": (c_int, [_P, c_int32, _I64, _I64, c_int32, _I64, c_double, c_int32,
                                         POINTER(c_double), POINTER(c_double)]),
     "hpspmm_ctx_tma_fallbacks": (c_int, [_P, POINTER(_I64)]),
+    "hpspmm_ctx_timeouts": (c_int, [_P, POINTER(_I64)]),
     "hpspmm_probe_tma_gather_gbs": (c_int, [_P, c_int32, _I64, _I64, c_int32, c_int32, POINTER(c_double),
                                             POINTER(c_double), POINTER(c_double), POINTER(_I64)]),
 }
@@ -511,6 +512,12 @@ class Context:
         """Warps of the HPSPMM_ALGO_TMA kernel that gave up waiting for a TMA copy (expected 0); synchronises."""
         n = _I64()
         self._check(self.lib.hpspmm_ctx_tma_fallbacks(self.handle, byref(n)), "hpspmm_ctx_tma_fallbacks")
+        return n.value
+
+    def timeouts(self):
+        """Blocks of the grouped products' tensor-core kernels that gave up a wait (expected 0); synchronises."""
+        n = _I64()
+        self._check(self.lib.hpspmm_ctx_timeouts(self.handle, byref(n)), "hpspmm_ctx_timeouts")
         return n.value
 
     def probe_tma_gather(self, row_bytes, table_rows, n_gathers, ctas_per_sm=2, repeats=10):

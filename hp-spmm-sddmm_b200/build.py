@@ -33,6 +33,7 @@ SOURCES = [
     "layer_grad_kernels.cu",
     "embedding_kernels.cu",
     "grouped_kernels.cu",
+    "grouped_tensor_kernels.cu",
     "distill_kernels.cu",
     "structure_kernels.cu",
     "graph_layer.cu",

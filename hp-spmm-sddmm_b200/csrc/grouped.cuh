@@ -1,0 +1,32 @@
+// Groups of rows: what the kernels of the grouped products share.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "device_utils.cuh"
+#include "hpspmm_internal.h"
+
+namespace hpspmm {
+
+// Bounds of part i of the rows: the groups, then the rows behind the last and in front of the first one.  Offsets are
+// taken into [0, R], so that whatever they hold no row outside the operands is named.
+__device__ __forceinline__ void part_bounds(const int* offsets, int G, int R, int i, int& begin, int& end) {
+  begin = end = 0;
+  if (i < G) {
+    begin = min(max(ld_chained(offsets + i), 0), R);
+    end = min(max(ld_chained(offsets + i + 1), 0), R);
+  } else if (i == G) {
+    begin = min(max(ld_chained(offsets + G), 0), R);
+    end = R;
+  } else if (i == G + 1) {
+    end = min(max(ld_chained(offsets), 0), R);
+  }
+}
+
+}  // namespace hpspmm
+
+// The tensor-core kernels.  0: launched, 1: the call is not for them (types, alignment), otherwise a status.
+int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx,
+                                  const void* W, bool out_first, const int32_t* offsets, void* Y, cudaStream_t s);
+int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t I, int64_t J, int32_t type, const void* A,
+                                      int64_t lda, const void* B, int64_t ldb, const int32_t* offsets, void* dW, cudaStream_t s);

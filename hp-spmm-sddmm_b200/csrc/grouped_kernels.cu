@@ -6,6 +6,7 @@
 
 #include "dense_types.cuh"
 #include "device_utils.cuh"
+#include "grouped.cuh"
 #include "hpspmm_internal.h"
 
 namespace {
@@ -18,21 +19,6 @@ constexpr int kThreads = 256;
 struct row_tile {
   int g, r0, rows;
 };
-
-// Bounds of part i of the rows: the groups, then the rows behind the last and in front of the first one.  Offsets are
-// taken into [0, R], so that whatever they hold no row outside the operands is named.
-__device__ __forceinline__ void part_bounds(const int* offsets, int G, int R, int i, int& begin, int& end) {
-  begin = end = 0;
-  if (i < G) {
-    begin = min(max(offsets[i], 0), R);
-    end = min(max(offsets[i + 1], 0), R);
-  } else if (i == G) {
-    begin = min(max(offsets[G], 0), R);
-    end = R;
-  } else if (i == G + 1) {
-    end = min(max(offsets[0], 0), R);
-  }
-}
 
 // The t-th tile of up to BM rows; called by one whole warp.  rows = 0: there is none.
 template <int BM>
@@ -177,10 +163,12 @@ int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int
   HPSPMM_REQUIRE(ctx, ldx >= 0, "negative row stride");
   if (R == 0 || N == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, offsets && Y && (K == 0 || (X && (W || G == 0))), "null pointer");
-  const int64_t col_tiles = (N + 63) / 64, blocks = ((R + 63) / 64 + G + 2) * col_tiles;
-  if (blocks > 2147483647ll) return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 64 x 64");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
+  const int done = hpspmm_grouped_product_tensor(ctx, R, G, K, N, type, X, ldx, W, w_out_first != 0, offsets, Y, s);
+  if (done != 1) return done;
+  const int64_t col_tiles = (N + 63) / 64, blocks = ((R + 63) / 64 + G + 2) * col_tiles;
+  if (blocks > 2147483647ll) return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 64 x 64");
   if (type == HPSPMM_TYPE_F32)
     launch_product<float>(R, G, K, N, X, ldx, W, w_out_first != 0, offsets, Y, (unsigned)blocks, (int)col_tiles, s);
   else if (type == HPSPMM_TYPE_F16)
@@ -207,6 +195,8 @@ int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K,
   const int64_t I = w_out_first ? N : K, J = w_out_first ? K : N;
   const void *A = w_out_first ? dY : X, *B = w_out_first ? X : dY;
   const int64_t lda = w_out_first ? ldy : ldx, ldb = w_out_first ? ldx : ldy;
+  const int done = hpspmm_grouped_weight_grad_tensor(ctx, R, G, I, J, type, A, lda, B, ldb, offsets, dW, s);
+  if (done != 1) return done;
   const int64_t i_tiles = (I + 63) / 64, j_tiles = (J + 63) / 64;
   if (i_tiles * j_tiles > 2147483647ll / G) return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 64 x 64");
   const unsigned blocks = (unsigned)(G * i_tiles * j_tiles);

@@ -1,0 +1,579 @@
+// Products of groups of rows on the tensor cores (16-bit types), and the gradient of their matrices.
+//
+//   Y[r]  = X[r] * W[g]     accumulator tile: 128 columns of Y (lanes) x up to BN rows of one group (columns)
+//   dW[g] = A_g^T * B_g     accumulator tile: 128 columns of dW (lanes) x up to BN rows of dW (columns)
+//
+// One warp issues TMA copies into a ring of swizzled tiles, one issues tcgen05.mma on them, four carry finished
+// accumulators from tensor memory to global memory while the next tile is multiplied into the other half.  The matrix (W)
+// sits on the 128-wide side of the instruction and the rows on its N side, which the instruction takes in steps of 16 up to
+// 256: a tile costs as much as the rows that its group has, whether that is one row or 256, and a lane's neighbours hold
+// neighbouring columns of Y, so that a warp's stores are contiguous.  Blocks stay for the whole call (one to an SM) and take
+// tiles in turn; the tiles follow from the offsets, which only the device knows.
+// Where the tiles are fewer than the SMs (a step of a decoder), clusters of 2 to 8 blocks split the depth of one tile and
+// add their parts through distributed shared memory, in the order of their ranks.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "dense_types.cuh"
+#include "device_utils.cuh"
+#include "grouped.cuh"
+
+namespace {
+
+using namespace hpspmm;
+
+constexpr int kThreads = 256;
+constexpr int kLanes = 128;                    // columns of the output to a tile
+constexpr int kDepth = 64;                     // of one stage: 128 bytes, the span of the swizzle
+constexpr int kABytes = kLanes * kDepth * 2;
+constexpr int kMaxGroups = 2048;               // of one launch: their tile counts lie in shared memory
+constexpr int kMaxTiles = 0x7fff0000;          // of one launch: adding a grid to it stays within 31 bits
+constexpr int kMostTiles = 1 << 29;            // where the sum of the groups' tiles stops: two of them are below 2^31
+
+enum { MODE_OUT_FIRST, MODE_IN_FIRST, MODE_WEIGHT };   // W stored [G, N, K], [G, K, N]; gradient of the matrices
+
+struct tensor_args {
+  const int* offsets;
+  int R, G;            // rows, groups of the call
+  int g0, gn;          // groups of this launch
+  int depth;           // products: K
+  int rows, cols;      // of the output: products: -, N; gradients: rows and columns of one matrix
+  int zero_rows;       // products: whether this launch clears the rows of no group
+  int* timeouts;
+};
+
+// ---- instructions ------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar, int rank) {
+  asm volatile(
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
+      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(bar), "r"(rank) : "memory");
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  if (CLUSTER)
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Waits for at most about two seconds.  Whoever gives up says so in `failed`, and all others give up with it.
+template <bool CLUSTER>
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* failed) {
+  const long long begin = clock64();
+  while (true) {
+    if (mbar_try<CLUSTER>(bar, parity)) return true;
+    if (*failed) return false;
+    if (clock64() - begin > 4000000000ll) {
+      *failed = 1;
+      return false;
+    }
+  }
+}
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+  return mbar_try<CLUSTER>(bar, parity) || mbar_wait_slow<CLUSTER>(bar, parity, failed);
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+               "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+               "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// Shared-memory operand, 128-byte swizzle.  Along the depth (LINES_OF_DEPTH: every 128-byte line holds 64 elements along
+// the depth): groups of 8 lines 1024 bytes apart.  Across it (a line holds 64 elements across the depth): 8 lines of depth
+// 1024 bytes apart, the next 64 elements across 64 lines = 8192 bytes further.
+template <bool LINES_OF_DEPTH>
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+  const uint64_t lead = LINES_OF_DEPTH ? 1 : (kDepth * 128) >> 4;
+  return (uint64_t)((addr & 0x3ffff) >> 4) | lead << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// 16 elements further along the depth, in the descriptor's units of 16 bytes
+template <bool LINES_OF_DEPTH>
+__device__ __forceinline__ constexpr uint64_t operand_step() { return LINES_OF_DEPTH ? 32 >> 4 : (16 * 128) >> 4; }
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a),
+               "l"(b), "r"(instr), "r"((int)add) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of the warp's 32 lanes
+__device__ __forceinline__ void tensor_load(uint32_t addr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// ---- tiles -------------------------------------------------------------------------------------------------------
+
+struct tile {
+  int g;               // group
+  int row0, rows;      // of the output, inside Y or inside the group's matrix
+  int col0;            // of the output
+  int begin, end;      // depth: products: stages of this block; gradients: rows of the group
+  int stages;
+};
+
+template <int MODE, int BN, int CL>
+__device__ __forceinline__ int tile_count(const tensor_args& a, const int* ends) {
+  const int across = (a.cols + kLanes - 1) / kLanes;
+  if (MODE == MODE_WEIGHT) return a.gn * ((a.rows + BN - 1) / BN) * across;
+  return (int)min((int64_t)ends[a.gn - 1] * across, (int64_t)kMaxTiles);
+}
+
+template <int MODE, int BN, int CL>
+__device__ __forceinline__ tile tile_at(const tensor_args& a, const int* ends, int u, int rank) {
+  tile t;
+  const int across = (a.cols + kLanes - 1) / kLanes;
+  const int q = u / across;
+  t.col0 = (u - q * across) * kLanes;
+  if (MODE == MODE_WEIGHT) {
+    const int down = (a.rows + BN - 1) / BN;
+    t.g = a.g0 + q / down;
+    t.row0 = (q % down) * BN;
+    t.rows = min(BN, a.rows - t.row0);
+    part_bounds(a.offsets, a.G, a.R, t.g, t.begin, t.end);
+    t.stages = (max(t.end - t.begin, 0) + kDepth - 1) / kDepth;
+    return t;
+  }
+  int lo = 0, hi = a.gn - 1;
+  while (lo < hi) {
+    const int m = (lo + hi) >> 1;
+    if (ends[m] > q) hi = m; else lo = m + 1;
+  }
+  t.g = a.g0 + lo;
+  const int first = lo ? ends[lo - 1] : 0, tiles = ends[lo] - first;
+  int begin, end;
+  part_bounds(a.offsets, a.G, a.R, t.g, begin, end);
+  // equal tiles, in steps of the instruction's 16; never more than BN rows, and as tiles = ceil(rows / BN), none is empty
+  // (offsets that do not ascend can have more rows than there are, and their count of tiles is cut off)
+  const int step = min(((end - begin + tiles - 1) / tiles + 15) / 16 * 16, BN);
+  t.row0 = begin + (q - first) * step;
+  t.rows = min(step, end - t.row0);
+  const int stages = (a.depth + kDepth - 1) / kDepth;
+  t.begin = CL == 1 ? 0 : (int)((int64_t)stages * rank / CL);
+  t.end = CL == 1 ? stages : (int)((int64_t)stages * (rank + 1) / CL);
+  t.stages = t.end - t.begin;
+  return t;
+}
+
+template <typename T>
+struct type_code;
+template <>
+struct type_code<__half> { static constexpr uint32_t value = 0; };
+template <>
+struct type_code<__nv_bfloat16> { static constexpr uint32_t value = 1; };
+
+// rows to a TMA box of the N-side operand: few where tiles are small, so that little is fetched for nothing
+template <int BN>
+__host__ __device__ constexpr int box_rows() { return BN >= 128 ? 64 : 16; }
+
+template <int BN, int STAGES, int CL>
+constexpr int smem_bytes() { return 1024 + STAGES * (kABytes + BN * 128) + (CL > 1 ? BN * kLanes * 4 : 0); }
+
+template <typename T, int MODE, int BN, int STAGES, int CL>
+__global__ void __launch_bounds__(kThreads, 1)
+grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                      T* __restrict__ out) {
+  constexpr bool kWeight = MODE == MODE_WEIGHT;
+  constexpr bool kALines = MODE == MODE_OUT_FIRST, kBLines = !kWeight;   // which operands have lines along the depth
+  constexpr int kBBytes = BN * 128, kStage = kABytes + kBBytes, kBox = box_rows<BN>();
+  constexpr int kColumns = 2 * BN < 32 ? 32 : 2 * BN;                   // of tensor memory: two accumulators
+  extern __shared__ char raw[];
+  __shared__ int ends[kMaxGroups];
+  __shared__ int part[kThreads / 32];
+  __shared__ uint64_t bars[2 * STAGES + 6];
+  __shared__ uint32_t tmem_base;
+  __shared__ int failed;
+  const uint32_t base = (smem_of(raw) + 1023) / 1024 * 1024;
+  const uint32_t bar0 = smem_of(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
+  const uint32_t parts_full = bar0 + 8u * (2 * STAGES + 4), parts_empty = bar0 + 8u * (2 * STAGES + 5);
+  float* const parts = reinterpret_cast<float*>(raw + (base - smem_of(raw)) + STAGES * kStage);   // [source][row][lane]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int rank = 0;
+  if (CL > 1) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+
+  if (threadIdx.x == 0) {
+    failed = 0;
+    for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+    for (int b = 0; b < 2; ++b) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 4);
+    mbar_init(parts_full, 4 * CL), mbar_init(parts_empty, 4 * CL);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&tmem_base)), "n"(kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tensor_fence_before();
+  }
+  chain_grid();
+
+  if (!kWeight) {   // how many tiles the groups up to each one have
+    constexpr int kPer = kMaxGroups / kThreads;
+    int n[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int g = threadIdx.x * kPer + i;
+      int begin = 0, end = 0;
+      if (g < a.gn) part_bounds(a.offsets, a.G, a.R, a.g0 + g, begin, end);
+      n[i] = (max(end - begin, 0) + BN - 1) / BN;
+      sum = min(sum + n[i], kMostTiles);
+    }
+    int before = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before = min(before + o, kMostTiles);
+    }
+    if (lane == 31) part[warp] = before;
+    __syncthreads();
+    before = max(before - sum, 0);
+    for (int w = 0; w < warp; ++w) before = min(before + part[w], kMostTiles);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      before = min(before + n[i], kMostTiles);
+      ends[threadIdx.x * kPer + i] = before;
+    }
+  }
+  __syncthreads();
+  if (CL > 1) {   // the others' barriers are ready
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  tensor_fence_after();
+  const uint32_t tmem = tmem_base;
+  const int units = tile_count<MODE, BN, CL>(a, ends);
+  const int first = blockIdx.x / CL, step = gridDim.x / CL;
+
+  if (warp == 0) {
+    if (lane == 0) {   // copies
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = first; u < units && ok; u += step) {
+        const tile t = tile_at<MODE, BN, CL>(a, ends, u, rank);
+        const int boxes = (t.rows + kBox - 1) / kBox;
+        for (int k = 0; k < t.stages; ++k) {
+          ok = mbar_wait(empty(s), phase ^ 1, &failed);
+          if (!ok) break;
+          const uint32_t dst = base + s * kStage, bar = full(s);
+          if (kWeight) {
+            const int wide = (t.rows + 63) / 64, r = t.begin + k * kDepth;
+            mbar_expect(bar, kABytes + wide * 8192);
+            tma_load(dst, &map_a, bar, t.col0, r);
+            tma_load(dst + 8192, &map_a, bar, t.col0 + 64, r);
+            for (int b = 0; b < wide; ++b) tma_load(dst + kABytes + b * 8192, &map_b, bar, t.row0 + b * 64, r);
+          } else {
+            const int d = (t.begin + k) * kDepth;
+            mbar_expect(bar, kABytes + boxes * kBox * 128);
+            if (MODE == MODE_OUT_FIRST) {
+              tma_load(dst, &map_a, bar, d, t.col0, t.g);
+            } else {
+              tma_load(dst, &map_a, bar, t.col0, d, t.g);
+              tma_load(dst + 8192, &map_a, bar, t.col0 + 64, d, t.g);
+            }
+            for (int b = 0; b < boxes; ++b) tma_load(dst + kABytes + b * kBox * 128, &map_b, bar, d, t.row0 + b * kBox);
+          }
+          if (++s == STAGES) s = 0, phase ^= 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {   // products
+    int s = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    for (int u = first; u < units; u += step) {
+      const tile t = tile_at<MODE, BN, CL>(a, ends, u, rank);
+      if (!mbar_wait(acc_empty(acc), acc_phase ^ 1, &failed)) break;
+      tensor_fence_after();
+      const uint32_t d = tmem + acc * BN;
+      const int n = (t.rows + 15) / 16 * 16;
+      // accumulate in 32 bits; type of A and B; whether their lines run across the depth; N / 8; M / 16
+      const uint32_t instr = 1u << 4 | type_code<T>::value << 7 | type_code<T>::value << 10 | (uint32_t)!kALines << 15 |
+                             (uint32_t)!kBLines << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(kLanes >> 4) << 24;
+      bool ok = true;
+      for (int k = 0; k < t.stages; ++k) {
+        ok = mbar_wait(full(s), phase, &failed);
+        if (!ok) break;
+        tensor_fence_after();
+        const uint32_t src = base + s * kStage;
+        int left;   // of the depth in this stage
+        if (kWeight) {
+          left = t.end - t.begin - k * kDepth;
+          if (left < kDepth && (left & 15)) {   // the next group's rows, up to the end of the instruction's depth, become zeros
+            const int wide = 2 + (t.rows + 63) / 64, rows = 16 - (left & 15);
+            for (int i = lane; i < wide * rows * 8; i += 32) {
+              const int b = i / (rows * 8), r = left + (i >> 3) % rows;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(src + b * 8192 + r * 128 + (i & 7) * 16), "r"(0) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        } else {
+          left = a.depth - (t.begin + k) * kDepth;
+        }
+        if (lane == 0) {
+          uint64_t da = operand<kALines>(src), db = operand<kBLines>(src + kABytes);
+          const int steps = min(kDepth / 16, (left + 15) / 16);
+          for (int i = 0; i < steps; ++i) {
+            mma(d, da, db, instr, k > 0 || i > 0);
+            da += operand_step<kALines>(), db += operand_step<kBLines>();
+          }
+          mma_commit(empty(s));
+        }
+        __syncwarp();
+        if (++s == STAGES) s = 0, phase ^= 1;
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        if (t.stages)
+          mma_commit(acc_full(acc));
+        else
+          mbar_arrive(acc_full(acc));
+      }
+      __syncwarp();
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+  } else if (warp >= 4) {   // results
+    const int q = warp - 4;
+    int acc = 0;
+    uint32_t acc_phase = 0, part_phase = 0;
+    for (int u = first; u < units; u += step) {
+      const tile t = tile_at<MODE, BN, CL>(a, ends, u, rank);
+      if (!mbar_wait(acc_full(acc), acc_phase, &failed)) break;
+      tensor_fence_after();
+      const uint32_t src = tmem + acc * BN + ((uint32_t)(q * 32) << 16);
+      const int col = t.col0 + q * 32 + lane;
+      const bool inside = col < a.cols;
+      T* to = out + (kWeight ? (int64_t)t.g * a.rows * a.cols : 0) + (int64_t)t.row0 * a.cols + col;
+      if (CL == 1) {
+        for (int c = 0; c < t.rows; c += 32) {
+          uint32_t v[32];
+          tensor_load(src + c, v);
+          if (kWeight && t.stages == 0) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (inside && c + j < t.rows) *to = from_float<T>(__uint_as_float(v[j]));
+            to += a.cols;
+          }
+        }
+        tensor_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty(acc));
+      } else {
+        // Every block takes 1 / CL of the tile's rows and gets the others' parts of them pushed into its shared memory.
+        const int share = (t.rows + 15) / 16 * 16 / CL;
+        if (!mbar_wait<true>(parts_empty, part_phase ^ 1, &failed)) break;
+        for (int c = 0; c < CL * share; c += 32) {
+          uint32_t v[32];
+          tensor_load(src + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (c + j < CL * share) {
+              const int to_rank = (c + j) / share, r = c + j - to_rank * share;
+              const uint32_t at = smem_of(parts + (rank * share + r) * kLanes + q * 32 + lane);
+              asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n st.shared::cluster.b32 [a], %2;\n}\n" ::"r"(at),
+                           "r"(to_rank), "r"(v[j]) : "memory");
+            }
+          }
+        }
+        tensor_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(acc_empty(acc));
+          for (int p = 0; p < CL; ++p) mbar_arrive_remote(parts_full, p);
+        }
+        __syncwarp();
+        if (!mbar_wait<true>(parts_full, part_phase, &failed)) break;
+        for (int r = 0; r < share; ++r) {
+          float sum = 0.f;
+#pragma unroll
+          for (int p = 0; p < CL; ++p) sum += parts[(p * share + r) * kLanes + q * 32 + lane];
+          const int row = rank * share + r;
+          if (inside && row < t.rows) to[(int64_t)row * a.cols] = from_float<T>(sum);
+        }
+        __syncwarp();
+        if (lane == 0)
+          for (int p = 0; p < CL; ++p) mbar_arrive_remote(parts_empty, p);
+        part_phase ^= 1;
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+  } else if (!kWeight && a.zero_rows) {   // rows of no group, by the two warps that are left
+    const int64_t width = a.cols / 8;     // 16-byte words to a row
+    uint4* words = reinterpret_cast<uint4*>(out);
+    const int64_t at = (int64_t)blockIdx.x * 64 + (threadIdx.x - 64), all = (int64_t)gridDim.x * 64;
+    for (int i = a.G; i < a.G + 2; ++i) {
+      int begin, end;
+      part_bounds(a.offsets, a.G, a.R, i, begin, end);
+      for (int64_t w = begin * width + at; w < end * width; w += all) words[w] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  tensor_fence_before();
+  __syncthreads();
+  if (failed) {   // what was started lands before the memory is given back
+    if (threadIdx.x == 0) atomicAdd(a.timeouts, 1);
+    const long long begin = clock64();
+    while (clock64() - begin < 4000000ll) __nanosleep(1000);
+  }
+  if (CL > 1) {   // nobody pushes into the memory of a block that has left
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  if (warp == 2) {
+    tensor_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kColumns) : "memory");
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------
+
+typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A dense array of 16-bit elements, innermost dimension first; strides in elements of all but the innermost.
+bool encode(CUtensorMap* map, bool half, const void* p, int dims, const int64_t* size, const int64_t* stride, const int* box) {
+  encode_fn fn = (encode_fn)hpspmm_tensor_map_encoder();
+  if (!fn) return false;
+  cuuint64_t sizes[3], strides[2];
+  cuuint32_t boxes[3], ones[3] = {1, 1, 1};
+  for (int i = 0; i < dims; ++i) sizes[i] = (cuuint64_t)size[i], boxes[i] = (cuuint32_t)box[i];
+  for (int i = 0; i + 1 < dims; ++i) {
+    if (stride[i] >= (int64_t)1 << 38) return false;
+    strides[i] = (cuuint64_t)stride[i] * 2;
+  }
+  return fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, const_cast<void*>(p), sizes, strides,
+            boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int MODE, int BN, int STAGES, int CL>
+cudaError_t launch_one(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* out, int64_t units,
+                       cudaStream_t s) {
+  auto* kernel = grouped_tensor_kernel<T, MODE, BN, STAGES, CL>;
+  constexpr int smem = smem_bytes<BN, STAGES, CL>();
+  // per call: the attribute belongs to the current device's context, and a process may drive several GPUs
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CL, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((unsigned)(std::min<int64_t>(units, ctx->sm_count / CL) * CL));
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = smem, c.stream = s, c.attrs = attr, c.numAttrs = CL > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&c, kernel, a, ma, mb, (T*)out);
+  ctx->launches++;
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <typename T, int MODE>
+cudaError_t launch_product(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* out, bool wide,
+                           int64_t units, cudaStream_t s) {
+  if (wide) return launch_one<T, MODE, 256, 4, 1>(ctx, a, ma, mb, out, units, s);
+  const int stages = (a.depth + kDepth - 1) / kDepth;
+  int cl = 8;
+  while (cl > 1 && (units * cl > ctx->sm_count || stages < 2 * cl)) cl /= 2;
+  if (cl == 8) return launch_one<T, MODE, 64, 7, 8>(ctx, a, ma, mb, out, units, s);
+  if (cl == 4) return launch_one<T, MODE, 64, 7, 4>(ctx, a, ma, mb, out, units, s);
+  if (cl == 2) return launch_one<T, MODE, 64, 7, 2>(ctx, a, ma, mb, out, units, s);
+  return launch_one<T, MODE, 64, 8, 1>(ctx, a, ma, mb, out, units, s);
+}
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+// 0: launched, 1: this path does not take the call, otherwise a status
+int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx,
+                                  const void* W, bool out_first, const int32_t* offsets, void* Y, cudaStream_t s) {
+  if (type == HPSPMM_TYPE_F32 || K % 8 || N % 8 || ldx % 8 || ldx < K || G == 0 || K == 0 || !aligned(X) || !aligned(W) || !aligned(Y))
+    return 1;
+  const bool half = type == HPSPMM_TYPE_F16;
+  const bool wide = R > 64 * G;
+  const int64_t bn = wide ? 256 : 64;
+  CUtensorMap ma, mb;
+  const int64_t wsize[3] = {out_first ? K : N, out_first ? N : K, G}, wstride[2] = {wsize[0], K * N};
+  const int wbox[3] = {64, out_first ? kLanes : kDepth, 1};
+  const int64_t xsize[2] = {K, R}, xstride[1] = {ldx};
+  const int xbox[2] = {kDepth, wide ? box_rows<256>() : box_rows<64>()};
+  if (!encode(&ma, half, W, 3, wsize, wstride, wbox) || !encode(&mb, half, X, 2, xsize, xstride, xbox)) return 1;
+  const int64_t across = (N + kLanes - 1) / kLanes;
+  if ((R / bn + G + 1) * across > kMaxTiles || R / bn + G + 1 > kMostTiles) return 1;
+  for (int64_t g0 = 0; g0 < G; g0 += kMaxGroups) {
+    const int64_t gn = std::min<int64_t>(kMaxGroups, G - g0);
+    const tensor_args a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
+    const int64_t units = (std::min(R, gn) + R / bn) * across;   // no more than that
+    cudaError_t e;
+    if (half)
+      e = out_first ? launch_product<__half, MODE_OUT_FIRST>(ctx, a, ma, mb, Y, wide, units, s)
+                    : launch_product<__half, MODE_IN_FIRST>(ctx, a, ma, mb, Y, wide, units, s);
+    else
+      e = out_first ? launch_product<__nv_bfloat16, MODE_OUT_FIRST>(ctx, a, ma, mb, Y, wide, units, s)
+                    : launch_product<__nv_bfloat16, MODE_IN_FIRST>(ctx, a, ma, mb, Y, wide, units, s);
+    HPSPMM_CUDA_TRY(ctx, e);
+  }
+  return HPSPMM_OK;
+}
+
+// dW[g] (I x J) = A_g^T * B_g with A R x I and B R x J
+int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t I, int64_t J, int32_t type, const void* A,
+                                      int64_t lda, const void* B, int64_t ldb, const int32_t* offsets, void* dW, cudaStream_t s) {
+  if (type == HPSPMM_TYPE_F32 || R == 0 || I % 8 || J % 8 || lda % 8 || ldb % 8 || lda < I || ldb < J || !aligned(A) || !aligned(B))
+    return 1;
+  const bool half = type == HPSPMM_TYPE_F16;
+  CUtensorMap ma, mb;   // the operand of the output's columns lies on the lanes
+  const int64_t asize[2] = {J, R}, astride[1] = {ldb}, bsize[2] = {I, R}, bstride[1] = {lda};
+  const int box[2] = {64, kDepth};
+  if (!encode(&ma, half, B, 2, asize, astride, box) || !encode(&mb, half, A, 2, bsize, bstride, box)) return 1;
+  const int64_t units = G * ((I + 255) / 256) * ((J + kLanes - 1) / kLanes);
+  if (units > kMaxTiles) return 1;
+  const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
+  const cudaError_t e = half ? launch_one<__half, MODE_WEIGHT, 256, 4, 1>(ctx, a, ma, mb, dW, units, s)
+                             : launch_one<__nv_bfloat16, MODE_WEIGHT, 256, 4, 1>(ctx, a, ma, mb, dW, units, s);
+  HPSPMM_CUDA_TRY(ctx, e);
+  return HPSPMM_OK;
+}

@@ -40,6 +40,9 @@ struct hpspmm_ctx {
 // ctx->flag[HPSPMM_FLAG_TMA_FALLBACKS] counts the warps of spmm_tma_kernel whose bounded wait for a TMA copy
 // ran out (they finish their chunk with ordinary loads); hpspmm_ctx_tma_fallbacks reads it.
 #define HPSPMM_FLAG_TMA_FALLBACKS 16
+// ctx->flag[HPSPMM_FLAG_TENSOR_TIMEOUTS] counts the blocks of grouped_tensor_kernel that gave up a wait;
+// hpspmm_ctx_timeouts reads it.
+#define HPSPMM_FLAG_TENSOR_TIMEOUTS 17
 
 // Chunk table of one sparsity structure.
 //   chunk_start[c]  first nnz of chunk c (n_chunks + 1 entries)
@@ -216,6 +219,9 @@ struct hpspmm_trace_range {
   hpspmm_trace_range& operator=(const hpspmm_trace_range&) = delete;
 };
 #define HPSPMM_TRACE(name) hpspmm_trace_range hpspmm_trace_range__(name)
+
+// the driver's cuTensorMapEncodeTiled, or null
+void* hpspmm_tensor_map_encoder();
 
 int hpspmm_ensure_scratch(hpspmm_ctx* ctx, size_t bytes);
 // the same for a caller that can do with less: HPSPMM_ERR_OOM leaves the scratch as it was

@@ -447,6 +447,12 @@ tensor_map_encode_fn tensor_map_encoder() {
   return fn;
 }
 
+}  // namespace
+
+void* hpspmm_tensor_map_encoder() { return (void*)tensor_map_encoder(); }
+
+namespace {
+
 // The K = 128 product with B fetched by TMA.  Returns 1 when this path cannot take the call (no encoder in
 // the driver, a chunk size beyond what the kernel stages, a B the tensor map refuses): the caller then runs
 // the ordinary kernel.  0 = launched, negative = error.

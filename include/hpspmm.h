@@ -598,6 +598,11 @@ HPSPMM_API int hpspmm_probe_gather_gbs(hpspmm_ctx* ctx, int32_t row_bytes, int64
  * count is a health check (expected: 0).  Synchronises the device. */
 HPSPMM_API int hpspmm_ctx_tma_fallbacks(hpspmm_ctx* ctx, int64_t* count);
 
+/* Number of blocks of the tensor-core kernels of the grouped products, since the context was created, that gave up a wait
+ * inside the kernel after about two seconds (expected: 0).  The outputs of such a call are not to be used.
+ * Synchronises the device. */
+HPSPMM_API int hpspmm_ctx_timeouts(hpspmm_ctx* ctx, int64_t* count);
+
 /* The same random rows through the tensor memory accelerator: producer warps fetch four rows per
  * instruction into shared memory (cp.async.bulk.tensor ... tile::gather4 on a tensor map of the table),
  * consumer warps read every delivered byte into registers.  row_bytes is 128, 256 or 512; the table is
