@@ -38,53 +38,430 @@ lookup_kernel(int64_t total, int per_row, int N, const void* __restrict__ ids, i
   }
 }
 
-// Place of every position in the order of (id, position): how many come before it.  Ids outside the table count as N.
+// ---- positions sorted by id ----------------------------------------------------------------------------------------
+//
+// Key of a position: its id, N where that lies outside the table.  The sort is stable, so that every row of the gradient
+// is a sum over ascending positions.
+
+__device__ __forceinline__ int key_of(const void* ids, int wide, int64_t at, int N) {
+  const int id = load_id(ids, wide, at, N);
+  return id >= 0 ? id : N;
+}
+
+// Up to kRankMost positions: every one counts how many come before it in the order of (key, position).  n^2 / 8 comparisons
+// of a thread's eighth of the keys, all in shared memory; one launch where the radix sort needs three or more.
+constexpr int kRankMost = 8192;
+
 __global__ void __launch_bounds__(kThreads)
-rank_kernel(int T, int N, const void* __restrict__ ids, int wide, int* __restrict__ key_out, int* __restrict__ pos_out) {
-  __shared__ int keys[kThreads];
-  const int t = blockIdx.x * kThreads + threadIdx.x;
-  int mine = N;
-  if (t < T) {
-    const int id = load_id(ids, wide, t, N);
-    if (id >= 0) mine = id;
-  }
+rank_kernel(int T, int N, const void* ids, int wide, int* key_out, int* pos_out) {
+  __shared__ int4 keys[kRankMost / 4];
+  chain_grid();
+  int* flat = reinterpret_cast<int*>(keys);
+  const int vectors = (T + 3) / 4;
+  for (int j = threadIdx.x; j < 4 * vectors; j += kThreads) flat[j] = j < T ? key_of(ids, wide, j, N) : 0x7fffffff;
+  __syncthreads();
+  const int t = blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3), sub = threadIdx.x & 7;
+  const int mine = flat[min(t, T - 1)], own = t / 4;
   int rank = 0;
-  for (int base = 0; base < T; base += kThreads) {
-    __syncthreads();
-    int k = 0x7fffffff;
-    if (base + (int)threadIdx.x < T) {
-      const int id = load_id(ids, wide, base + threadIdx.x, N);
-      k = id >= 0 ? id : N;
-    }
-    keys[threadIdx.x] = k;
-    __syncthreads();
-    const int n = min(kThreads, T - base);
-    for (int j = 0; j < n; ++j) rank += keys[j] < mine || (keys[j] == mine && base + j < t);
+  for (int v = sub; v < vectors; v += 8) {
+    const int4 k = keys[v];
+    const int below = v < own ? mine + 1 : mine;   // in front of the position equal keys count, behind it they do not
+    rank += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
   }
-  if (t < T) {
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+  if (t < T && sub == 0) {
+    for (int j = own * 4; j < t; ++j) rank += flat[j] == mine;
     key_out[rank] = mine;
     pos_out[rank] = t;
   }
 }
 
-// One warp to a row of the table: the sorted positions of its id, in ascending order.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-sum_rows_kernel(int T_, int N, int K, const int* __restrict__ keys, const int* __restrict__ pos, const T* __restrict__ dout,
-                int64_t ld, float scale, T* __restrict__ dtable) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t v = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5; v < N; v += ((int64_t)gridDim.x * kThreads) >> 5) {
-    int lo = 0, hi = T_;
-    while (lo < hi) {
-      const int m = lo + (hi - lo) / 2;
-      if (keys[m] < v) lo = m + 1; else hi = m;
+// Radix sort by digits of up to 9 bits, for more positions.  Block b of each pass has the positions [b * chunk, ...).
+constexpr int kDigits = 512;
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortBlocks = 148;      // at most
+constexpr int kSortChunk = 2048;      // positions to a block, at least
+
+// Counts of the first digit; the tables of the later ones, which the passes in front of them fill, are cleared.
+__global__ void __launch_bounds__(kSortThreads)
+digit_count_kernel(int64_t T, int N, const void* ids, int wide, int64_t chunk, int digit_mask, int passes, int* tables) {
+  __shared__ int count[kDigits];
+  chain_grid();
+  count[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t end = min(T, (blockIdx.x + 1) * chunk);
+  for (int64_t t = blockIdx.x * chunk + threadIdx.x; t < end; t += kSortThreads)
+    atomicAdd(count + (key_of(ids, wide, t, N) & digit_mask), 1);
+  __syncthreads();
+  tables[blockIdx.x * kDigits + threadIdx.x] = count[threadIdx.x];
+  for (int p = 1; p < passes; ++p) tables[((int64_t)p * gridDim.x + blockIdx.x) * kDigits + threadIdx.x] = 0;
+}
+
+// One pass: positions to their places by one digit, in order within a digit.  keys_in is null in the first pass, which
+// reads the ids.  next: the counts of the next digit by block of the new order, or null in the last pass.
+__global__ void __launch_bounds__(kSortThreads)
+digit_place_kernel(int64_t T, int N, const void* ids, int wide, const int* keys_in, const int* pos_in, int64_t chunk, int shift,
+                   int digit_mask, int next_shift, const int* table, int* next, int* keys_out, int* pos_out) {
+  __shared__ int place[kSortWarps][kDigits];
+  __shared__ int of_digit[kDigits], of_digit_before[kDigits];
+  __shared__ int warp_sum[kSortWarps];
+  chain_grid();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto key_at = [&](int64_t t) { return keys_in ? keys_in[t] : key_of(ids, wide, t, N); };
+  of_digit[threadIdx.x] = of_digit_before[threadIdx.x] = 0;
+  __syncthreads();
+  {   // of every digit: how many there are, and how many in the blocks in front of this one
+    const int quad = threadIdx.x & 127, group = threadIdx.x >> 7;
+    int4 all = make_int4(0, 0, 0, 0), before = all;
+#pragma unroll 4
+    for (int b = group; b < gridDim.x; b += 4) {
+      const int4 c = reinterpret_cast<const int4*>(table)[b * (kDigits / 4) + quad];
+      all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
+      if (b < blockIdx.x) before.x += c.x, before.y += c.y, before.z += c.z, before.w += c.w;
     }
-    for (int c = lane; c < K; c += 32) {
-      float sum = 0.f;
-      for (int j = lo; j < T_ && keys[j] == v; ++j) sum += to_float(dout[pos[j] * ld + c]);
-      dtable[v * K + c] = from_float<T>(scale * sum);
+    int *to = of_digit + quad * 4, *to_before = of_digit_before + quad * 4;
+    atomicAdd(to, all.x), atomicAdd(to + 1, all.y), atomicAdd(to + 2, all.z), atomicAdd(to + 3, all.w);
+    atomicAdd(to_before, before.x), atomicAdd(to_before + 1, before.y), atomicAdd(to_before + 2, before.z), atomicAdd(to_before + 3, before.w);
+  }
+  const int64_t begin = blockIdx.x * chunk, end = min(T, begin + chunk);
+  const int64_t sub = (chunk / kSortWarps + 31) / 32 * 32;
+  const int64_t from = min(end, begin + warp * sub), to = min(end, from + sub);
+  for (int d = lane; d < kDigits; d += 32) place[warp][d] = 0;
+  __syncwarp();
+  for (int64_t t = from + lane; t < to; t += 32) atomicAdd(&place[warp][key_at(t) >> shift & digit_mask], 1);
+  __syncthreads();
+  {   // places of every warp's digits
+    const int d = threadIdx.x;
+    const int all = of_digit[d], before = of_digit_before[d];
+    int sum = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31) warp_sum[warp] = sum;
+    __syncthreads();
+    int at = sum - all + before;
+    for (int w = 0; w < warp; ++w) at += warp_sum[w];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int n = place[w][d];
+      place[w][d] = at;
+      at += n;
     }
   }
+  __syncthreads();
+  for (int64_t t0 = from; t0 < to; t0 += 32) {
+    const int64_t t = t0 + lane;
+    const bool have = t < to;
+    const int key = have ? key_at(t) : 0;
+    const int d = have ? key >> shift & digit_mask : kDigits;
+    const unsigned same = __match_any_sync(0xffffffffu, d);
+    const int before = __popc(same & ((1u << lane) - 1));
+    int at = 0;
+    if (have) at = place[warp][d] + before;
+    __syncwarp();
+    if (have) {
+      if (before == 0) place[warp][d] = at + __popc(same);
+      keys_out[at] = key;
+      pos_out[at] = pos_in ? pos_in[t] : (int)t;
+      if (next) atomicAdd(next + at / chunk * kDigits + (key >> next_shift & digit_mask), 1);
+    }
+    __syncwarp();
+  }
+}
+
+// ---- sums of sorted rows -------------------------------------------------------------------------------------------
+//
+// The work is the sorted positions (a row of dOut to read each) and the rows of the table (one to write each) in one
+// sequence: the positions of row 0, the end of row 0, the positions of row 1, ...  Position j of the sorted order comes at
+// place j + key[j], so a cut of the sequence into equal parts is found by a search, whatever the ids are: a table that is
+// all but empty is cleared at the speed of its stores, and an id that half of the batch names is shared by as many groups
+// of lanes as it has parts.  A group of W lanes takes one part of one slab of columns.  Rows that lie in several parts go to
+// `split` in 32 bits ([part][0: end of a row that began earlier, 1: beginning of a row that ends later][column]) and are
+// added up by the kernel behind, in the order of the parts.
+
+// number of positions in the sequence's first `d` places
+template <int W>
+__device__ __forceinline__ int positions_before(const int* keys, int T, int64_t d) {
+  const int lane = threadIdx.x & (W - 1);
+  const unsigned mask = subwarp_mask<W>();
+  const int shift = (threadIdx.x & 31) & ~(W - 1);
+  int lo = 0, n = T;   // the answer lies in [lo, lo + n]
+  while (n > 0) {
+    const int step = n / (W + 1) + 1;   // probes at lo + step - 1, lo + 2 * step - 1, ...
+    const int64_t j = (int64_t)lo + (int64_t)(lane + 1) * step - 1;
+    const bool inside = j < (int64_t)lo + n && j + keys[j] < d;
+    const int c = __popc(__ballot_sync(mask, inside) >> shift & (W == 32 ? 0xffffffffu : (1u << W) - 1));
+    const int used = c * step;
+    lo += used;
+    n = min(n - used, step - 1);
+  }
+  return lo;
+}
+
+template <typename T, int BYTES, int R, int W>
+__global__ void __launch_bounds__(kThreads)
+sum_parts_kernel(int n, int N, int K, int64_t parts, int slabs, int length, const int* keys, const int* pos,
+                 const T* __restrict__ dout, int64_t ld, float scale, T* __restrict__ dtable, int2* info, float* split) {
+  typedef dense_vec<T, BYTES> vec;
+  constexpr int E = vec::kCount;
+  constexpr int U = R >= 4 ? 2 : 4;     // rows of dOut in flight
+  chain_grid();
+  const int lane = threadIdx.x & (W - 1);
+  const unsigned mask = subwarp_mask<W>();
+  const int64_t id = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / W;
+  const int64_t part = id / slabs;
+  const int slab = (int)(id - part * slabs);
+  if (part >= parts) return;            // whole groups of lanes: nothing below reaches across them
+  const int64_t d0 = part * length, d1 = d0 + length;
+  int j = positions_before<W>(keys, n, d0);
+  int row = (int)min(d0 - j, (int64_t)N);
+  bool open = j > 0 && row < N && keys[j - 1] == row;     // the row began in an earlier part
+  if (slab == 0 && lane == 0) info[part] = make_int2(row, open);
+  int col[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) col[r] = (slab * R + r) * W * E + lane * E;
+  float acc[R][E];
+  auto clear = [&]() {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[r][e] = 0.f;
+  };
+  auto to_split = [&](int which) {
+    float* p = split + (2 * part + which) * K;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (col[r] < K) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) p[col[r] + e] = acc[r][e];
+      }
+  };
+  auto end_row = [&]() {
+    if (open) {
+      to_split(0);
+      open = false;
+    } else {
+      T* p = dtable + (int64_t)row * K;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (col[r] < K) {
+          vec v;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v.at[e] = from_float<T>(scale * acc[r][e]);
+          *reinterpret_cast<decltype(v.raw)*>(p + col[r]) = v.raw;
+        }
+    }
+    clear();
+    ++row;
+  };
+  clear();
+  bool last_is_row = true;   // the part's last place is the end of a row
+  while (true) {
+    // up to W positions of this part
+    const int64_t at = (int64_t)j + lane;
+    int key = 0x7fffffff, p = 0;
+    if (at < n) key = keys[at], p = pos[at];
+    const bool mine = at < n && key < N && at + key < d1;
+    const int have = __popc(__ballot_sync(mask, mine));    // the first ones: places ascend
+    for (int i = 0; i < have; i += U) {
+      vec v[U][R];
+      int k[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int l = min(i + u, have - 1);
+        k[u] = __shfl_sync(mask, key, l, W);
+        const T* src = dout + (int64_t)__shfl_sync(mask, p, l, W) * ld;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (i + u < have && col[r] < K) v[u][r].raw = *reinterpret_cast<const decltype(v[u][r].raw)*>(src + col[r]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u < have) {
+          while (row < k[u]) end_row();
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[r][e] += to_float(v[u][r].at[e]);
+        }
+      }
+    }
+    j += have;
+    if (have) last_is_row = false;
+    if (have < W) break;
+  }
+  const int last = (int)min(d1 - j, (int64_t)N);   // rows that end in front of the next part
+  if (row < last) last_is_row = true;
+  while (row < last) end_row();
+  if (!last_is_row) to_split(1);
+}
+
+// Rows that lie in several parts.  A block looks at 8 parts, one to a warp: a row that began earlier and ends in the part is
+// the sum of the pieces before it and its own; many pieces are shared by the block's warps.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+join_parts_kernel(int N, int K, int64_t parts, const int2* info, const float* split, float scale, T* __restrict__ dtable) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ int64_t first_of[kWarps];
+  __shared__ int row_of[kWarps];
+  __shared__ float sums[kWarps][32];
+  chain_grid();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t part = (int64_t)blockIdx.x * kWarps + warp;
+  int row = -1;
+  int64_t first = 0;
+  if (part < parts) {
+    const int2 here = info[part];
+    const int next = part + 1 < parts ? info[part + 1].x : N;
+    if (here.y && here.x < N && next > here.x) {
+      row = here.x;
+      int64_t lo = 0, n = part;   // first part that begins inside this row or at its first position: in [lo, lo + n]
+      while (n > 0) {
+        const int64_t step = n / 33 + 1, at = lo + (lane + 1) * step - 1;
+        const bool before = at < lo + n && info[at].x < row;
+        const int c = __popc(__ballot_sync(0xffffffffu, before));
+        lo += c * step;
+        n = min(n - c * step, step - 1);
+      }
+      first = info[lo].y ? lo - 1 : lo;   // (open: its beginning is the part in front)
+    }
+  }
+  if (lane == 0) row_of[warp] = row, first_of[warp] = first;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    const int r = row_of[w];
+    if (r < 0) continue;
+    const int64_t f = first_of[w], mine = (int64_t)blockIdx.x * kWarps + w, pieces = mine - f;
+    T* to = dtable + (int64_t)r * K;
+    if (pieces <= 2 * kWarps) {
+      for (int c = threadIdx.x; c < K; c += kThreads) {
+        float sum = 0.f;
+        for (int64_t s = f; s < mine; ++s) sum += split[(2 * s + 1) * K + c];
+        to[c] = from_float<T>(scale * (sum + split[2 * mine * K + c]));
+      }
+    } else {
+      const int64_t b = f + pieces * warp / kWarps, e = f + pieces * (warp + 1) / kWarps;
+      for (int c0 = 0; c0 < K; c0 += 32) {
+        const int c = c0 + lane;
+        float sum = 0.f;
+        if (c < K) {
+#pragma unroll 8
+          for (int64_t s = b; s < e; ++s) sum += split[(2 * s + 1) * K + c];
+        }
+        sums[warp][lane] = sum;
+        __syncthreads();
+        if (warp == 0 && c < K) {
+          sum = sums[0][lane];
+#pragma unroll
+          for (int i = 1; i < kWarps; ++i) sum += sums[i][lane];
+          to[c] = from_float<T>(scale * (sum + split[2 * mine * K + c]));
+        }
+        __syncthreads();
+      }
+    }
+  }
+}
+
+inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+// How a call of these sizes is cut up, and where its workspace lies.
+struct backward_plan {
+  int bits, passes;             // of the radix sort; passes = 0: the positions are ranked
+  int64_t chunk;
+  int blocks;
+  int length;                   // places to a part
+  int64_t parts;
+  size_t keys, pos, tables, info, split, bytes;   // offsets
+};
+
+// Places to a part: 64 amortise the search (4 rounds of 32 probes), 16 where there would be less than about a wave.
+backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
+  backward_plan p = {};
+  while (p.bits < 31 && ((int64_t)1 << p.bits) <= N) ++p.bits;
+  if (T > kRankMost) {
+    p.passes = (p.bits + 8) / 9;
+    p.bits = (p.bits + p.passes - 1) / p.passes;
+  }
+  p.chunk = std::max<int64_t>(kSortChunk, (T + kSortBlocks - 1) / kSortBlocks);
+  p.chunk = (p.chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
+  p.blocks = (int)((T + p.chunk - 1) / p.chunk);
+  p.length = (T + N) * ((K + 255) / 256) < 148 * 32 * 64 ? 16 : 64;
+  p.parts = (T + N + p.length - 1) / p.length;
+  const size_t b_t = align_up((size_t)T * 4, 256);
+  p.keys = 0;
+  p.pos = p.keys + b_t * (p.passes > 1 ? 2 : 1);
+  p.tables = p.pos + b_t * (p.passes > 1 ? 2 : 1);
+  p.info = p.tables + align_up((size_t)p.passes * p.blocks * kDigits * 4, 256);
+  p.split = p.info + align_up((size_t)p.parts * sizeof(int2), 256);
+  p.bytes = p.split + (size_t)p.parts * 2 * K * 4;
+  return p;
+}
+
+// Sorts; *keys and *pos point to the result.
+void launch_sort(hpspmm_ctx* ctx, const backward_plan& p, int64_t T, int64_t N, const void* ids, int wide, char* space,
+                 const int** keys, const int** pos, cudaStream_t s) {
+  const size_t b_t = align_up((size_t)T * 4, 256);
+  int *k = (int*)(space + p.keys), *at = (int*)(space + p.pos);
+  *keys = k, *pos = at;
+  if (p.passes == 0) {
+    hpspmm_launch(rank_kernel, dim3((unsigned)((T + kThreads / 8 - 1) / (kThreads / 8))), dim3(kThreads), 0, s, (int)T, (int)N, ids, wide,
+                  k, at);
+    ctx->launches++;
+    return;
+  }
+  int* tables = (int*)(space + p.tables);
+  const int mask = (1 << p.bits) - 1;
+  hpspmm_launch(digit_count_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, T, (int)N, ids, wide, p.chunk, mask, p.passes, tables);
+  ctx->launches++;
+  for (int i = 0; i < p.passes; ++i) {
+    // the last pass writes the first buffers
+    int* to_k = (p.passes - 1 - i) % 2 ? (int*)((char*)k + b_t) : k;
+    int* to_p = (p.passes - 1 - i) % 2 ? (int*)((char*)at + b_t) : at;
+    const int* from_k = i == 0 ? nullptr : (to_k == k ? (int*)((char*)k + b_t) : k);
+    const int* from_p = i == 0 ? nullptr : (to_p == at ? (int*)((char*)at + b_t) : at);
+    const int64_t table = (int64_t)p.blocks * kDigits;
+    hpspmm_launch(digit_place_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, T, (int)N, ids, wide, from_k, from_p, p.chunk, i * p.bits,
+                  mask, (i + 1) * p.bits, tables + i * table, i + 1 < p.passes ? tables + (i + 1) * table : nullptr, to_k, to_p);
+    ctx->launches++;
+  }
+}
+
+template <typename T, int BYTES, int R, int W>
+void launch_sums(hpspmm_ctx* ctx, const backward_plan& p, int64_t n, int64_t N, int64_t K, const int* keys, const int* pos,
+                 const void* dout, int64_t ld, float scale, void* dtable, char* space, cudaStream_t s) {
+  constexpr int kSlab = W * R * BYTES / (int)sizeof(T);
+  const int64_t slabs = (K + kSlab - 1) / kSlab, lanes = p.parts * slabs * W;
+  hpspmm_launch(sum_parts_kernel<T, BYTES, R, W>, dim3((unsigned)((lanes + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, (int)n, (int)N,
+                (int)K, p.parts, (int)slabs, p.length, keys, pos, (const T*)dout, ld, scale, (T*)dtable, (int2*)(space + p.info),
+                (float*)(space + p.split));
+  hpspmm_launch(join_parts_kernel<T>, dim3((unsigned)((p.parts + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads), 0, s, (int)N, (int)K,
+                p.parts, (const int2*)(space + p.info), (const float*)(space + p.split), scale, (T*)dtable);
+  ctx->launches += 2;
+}
+
+template <typename T>
+void launch_sums_of(hpspmm_ctx* ctx, const backward_plan& p, int64_t n, int64_t N, int64_t K, const int* keys, const int* pos,
+                    const void* dout, int64_t ld, float scale, void* dtable, char* space, cudaStream_t s) {
+  const int bytes = dense_vector_bytes((uintptr_t)dout | (uintptr_t)dtable | (uintptr_t)(K * (int64_t)sizeof(T)) |
+                                           (uintptr_t)(ld * (int64_t)sizeof(T)), (int)sizeof(T));
+  // 8 lanes to a group for rows of up to 8 vectors; four vectors to a lane where they are short
+  const bool narrow = K * (int64_t)sizeof(T) <= 8 * bytes;
+#define HPSPMM_SUMS(B, R)                                                                               \
+  (narrow ? launch_sums<T, B, 1, 8>(ctx, p, n, N, K, keys, pos, dout, ld, scale, dtable, space, s)     \
+          : launch_sums<T, B, R, 32>(ctx, p, n, N, K, keys, pos, dout, ld, scale, dtable, space, s))
+  if (bytes == 16)
+    HPSPMM_SUMS(16, 1);
+  else if (bytes == 8)
+    HPSPMM_SUMS(8, 2);
+  else if (bytes == 4 || sizeof(T) == 4)
+    HPSPMM_SUMS(4, 4);
+  else
+    HPSPMM_SUMS(sizeof(T), 4);
+#undef HPSPMM_SUMS
 }
 
 template <typename T, int BYTES>
@@ -123,8 +500,6 @@ int check_embedding(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, int32_t ty
   return HPSPMM_OK;
 }
 
-inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-
 }  // namespace
 
 extern "C" {
@@ -153,7 +528,7 @@ int hpspmm_embedding_forward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, i
 
 int64_t hpspmm_embedding_backward_workspace(int64_t T, int64_t N, int64_t K) {
   if (T < 0 || N < 0 || K < 0 || T > 2147483646ll || N > 2147483646ll || K > 2147483646ll) return -1;
-  return (int64_t)(2 * align_up((size_t)T * 4, 256));
+  return (int64_t)plan_backward(T, N, K).bytes;
 }
 
 int hpspmm_embedding_backward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, int32_t type, const void* ids,
@@ -164,25 +539,25 @@ int hpspmm_embedding_backward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, 
   if (st != HPSPMM_OK) return st;
   if (N == 0 || K == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, dTable && (T == 0 || (ids && dOut && workspace)), "null pointer");
-  HPSPMM_REQUIRE(ctx, (int64_t)workspace_bytes >= hpspmm_embedding_backward_workspace(T, N, K), "workspace too small");
+  const backward_plan p = plan_backward(T, N, K);
+  HPSPMM_REQUIRE(ctx, T == 0 || workspace_bytes >= p.bytes, "workspace too small");
+  HPSPMM_REQUIRE(ctx, T == 0 || ((uintptr_t)workspace & 255) == 0, "workspace not aligned to 256 bytes");
+  if (p.parts * ((K + 31) / 32) > (int64_t)2147483647 * 8) return hpspmm_unsupported(ctx, "more than 2^31 - 1 blocks");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
-  int* keys = (int*)workspace;
-  int* pos = (int*)((char*)workspace + align_up((size_t)T * 4, 256));
-  if (T > 0) {
-    rank_kernel<<<(unsigned)((T + kThreads - 1) / kThreads), kThreads, 0, s>>>((int)T, (int)N, ids, id_bytes == 8, keys, pos);
-    ctx->launches++;
-    HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
+  if (T == 0) {
+    HPSPMM_CUDA_TRY(ctx, cudaMemsetAsync(dTable, 0, (size_t)(N * K) * hpspmm::dense_type_size(type), s));
+    return HPSPMM_OK;
   }
-  const unsigned blocks = (unsigned)std::min<int64_t>((N + 7) / 8, (int64_t)ctx->sm_count * 64);
+  char* space = (char*)workspace;
+  const int *keys, *pos;
+  launch_sort(ctx, p, T, N, ids, id_bytes == 8, space, &keys, &pos, s);
   if (type == HPSPMM_TYPE_F32)
-    sum_rows_kernel<<<blocks, kThreads, 0, s>>>((int)T, (int)N, (int)K, keys, pos, (const float*)dOut, ld_dout, scale, (float*)dTable);
+    launch_sums_of<float>(ctx, p, T, N, K, keys, pos, dOut, ld_dout, scale, dTable, space, s);
   else if (type == HPSPMM_TYPE_F16)
-    sum_rows_kernel<<<blocks, kThreads, 0, s>>>((int)T, (int)N, (int)K, keys, pos, (const __half*)dOut, ld_dout, scale, (__half*)dTable);
+    launch_sums_of<__half>(ctx, p, T, N, K, keys, pos, dOut, ld_dout, scale, dTable, space, s);
   else
-    sum_rows_kernel<<<blocks, kThreads, 0, s>>>((int)T, (int)N, (int)K, keys, pos, (const __nv_bfloat16*)dOut, ld_dout, scale,
-                                                (__nv_bfloat16*)dTable);
-  ctx->launches++;
+    launch_sums_of<__nv_bfloat16>(ctx, p, T, N, K, keys, pos, dOut, ld_dout, scale, dTable, space, s);
   HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
   return HPSPMM_OK;
 }
