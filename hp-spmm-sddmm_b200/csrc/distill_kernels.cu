@@ -15,143 +15,325 @@ namespace {
 using namespace hpspmm;
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxEntries = 1024;   // of the teacher for one row
+constexpr int kMaxEntriesWarp = 64; // where a warp has a row
+constexpr int kVectors = 4;         // of 16 bytes in flight per thread
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// (within 2^-22 of the value; results below 2^-126 are zero)
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
+struct maximum {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct sum {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+
+// Over the NT threads that share a row: the same value in all of them.  part: one float for each warp.
+template <int NT, typename OP>
+__device__ __forceinline__ float row_reduce(float v, OP op, float* part) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
-}
-// the same value in every thread; `part` holds one float for each warp
-__device__ __forceinline__ float block_max(float v, float* part) {
-  v = warp_max(v);
+  for (int d = 16; d > 0; d >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, d));
+  if (NT == 32) return v;
   __syncthreads();
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   v = part[0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) v = fmaxf(v, part[w]);
+  for (int w = 1; w < NT / 32; ++w) v = op(v, part[w]);
   return v;
 }
-__device__ __forceinline__ float block_sum(float v, float* part) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = part[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) v += part[w];
-  return v;
+template <int NT>
+__device__ __forceinline__ void row_sync() {
+  if (NT == 32) __syncwarp(); else __syncthreads();
 }
+template <int NT>
+__device__ __forceinline__ bool row_any(bool v) { return NT == 32 ? __any_sync(0xffffffffu, v) : __syncthreads_or(v); }
 
-// The teacher's entries of one row: ids (-1: does not count) and exp((t - max) / tau).  Returns how many count, with the
-// largest logit and the sum of the exponentials, the same in every thread.
-__device__ __forceinline__ bool load_teacher(const void* ids, int wide, const float* teacher, int64_t at, int k, int V, float c,
-                                             int* id, float* e, float* part, float& top, float& total) {
-  float m = -INFINITY;
-  int count = 0;
-  for (int j = threadIdx.x; j < k; j += kThreads) {
-    const float t = teacher[at + j];
-    int i = load_id(ids, wide, at + j, V);
-    if (t == -INFINITY) i = -1;
-    id[j] = i;
-    e[j] = t;
-    if (i >= 0) m = fmaxf(m, t), ++count;
-  }
-  top = block_max(m, part);
-  const bool some = __syncthreads_or(count > 0);
-  float s = 0.f;
-  for (int j = threadIdx.x; j < k; j += kThreads) {
-    const float v = id[j] >= 0 ? exp2_fast((e[j] - top) * c) : 0.f;
-    e[j] = v;
-    s += v;
-  }
-  total = block_sum(s, part);   // (its barriers order the writes to e as well)
-  return some;
-}
-
+// A row of V elements at any address: `head` elements in front of the first 16-byte boundary, vectors, the rest from `tail` on.
 template <typename T>
+struct row_parts {
+  int head, vectors, tail;
+  __device__ __forceinline__ row_parts(const T* p, int V) {
+    constexpr int E = 16 / (int)sizeof(T);
+    head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T));
+    vectors = (V - head) / E;
+    tail = head + vectors * E;
+  }
+};
+
+// Largest value so far and the sum of exp((x - it) / tau) under it.
+struct running {
+  float top = -INFINITY, total = 0.f;
+  // where nothing has been seen but -infinity, the difference would be no number
+  static __device__ __forceinline__ float base(float top) { return top == -INFINITY ? 0.f : top; }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float c) {
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
+    if (most > top) {
+      total *= exp2_fast((top - most) * c);
+      top = most;
+    }
+    const float b = base(top);
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i & 3] += exp2_fast((x[i] - b) * c);
+    total += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+  __device__ __forceinline__ void add(float x, float c) {
+    const float v[1] = {x};
+    add(v, c);
+  }
+  // seen under a larger value
+  __device__ __forceinline__ float under(float most, float c) const {
+    return top == -INFINITY ? total : total * exp2_fast((top - most) * c);
+  }
+};
+
+// One pass over the row, everything in registers: NT threads to a row, CL blocks of a cluster to one where rows are few.
+// Bound by the reads of the logits; an element costs one ex2 and about five other instructions.
+template <typename T, int NT, int CL>
 __global__ void __launch_bounds__(kThreads)
-distill_forward_kernel(int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
+distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
                        const float* __restrict__ teacher, float tau, float* __restrict__ loss, float2* __restrict__ stats) {
-  __shared__ int id[kMaxEntries];
-  __shared__ float e[kMaxEntries], part[kWarps];
-  const int64_t row = blockIdx.x;
+  typedef dense_vec<T, 16> vec;
+  constexpr int E = vec::kCount;
+  constexpr int kRows = kThreads / NT, kEntries = NT == 32 ? kMaxEntriesWarp : kMaxEntries;
+  __shared__ float of_teacher[kRows][kEntries], of_student[kRows][kEntries];   // logits at the teacher's entries
+  __shared__ float part[kThreads / 32];
+  __shared__ float2 from_rank[CL];
+  const int tid = threadIdx.x & (NT - 1), slot = NT == 32 ? threadIdx.x >> 5 : 0;
+  const int rank = CL == 1 ? 0 : blockIdx.x & (CL - 1);
+  const int64_t row = CL == 1 ? (int64_t)blockIdx.x * kRows + slot : blockIdx.x / CL;
+  if (row >= rows) return;              // whole warps, and none of them in front of a barrier of the block
   const T* z = logits + row * ld;
   const float c = kLog2e / tau;
-  float m = -INFINITY, s = 0.f;
-  for (int v = threadIdx.x; v < V; v += kThreads) {
-    const float x = to_float(z[v]);
-    if (x > m) {
-      s *= exp2_fast((m - x) * c);
-      m = x;
+  if (rank == 0)
+    for (int j = tid; j < k; j += NT) {   // an entry that does not count: -infinity
+      const int id = load_id(ids, wide, row * k + j, V);
+      of_teacher[slot][j] = id >= 0 ? teacher[row * k + j] : -INFINITY;
+      of_student[slot][j] = id >= 0 ? to_float(z[id]) : 0.f;
     }
-    s += exp2_fast((x - (m == -INFINITY ? 0.f : m)) * c);
+  const row_parts<T> at(z, V);
+  running r;
+  if (rank == 0)
+    for (int v = tid; v < at.head; v += NT) r.add(to_float(z[v]), c);
+  if (rank == CL - 1)
+    for (int v = at.tail + tid; v < V; v += NT) r.add(to_float(z[v]), c);
+  const uint4* words = reinterpret_cast<const uint4*>(z + at.head);
+  const int begin = (int)((int64_t)at.vectors * rank / CL), end = (int)((int64_t)at.vectors * (rank + 1) / CL);
+  int v = begin + tid;
+  for (; v + (kVectors - 1) * NT < end; v += kVectors * NT) {
+    vec x[kVectors];
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u) x[u].raw = __ldg(words + v + u * NT);
+#pragma unroll
+    for (int u = 0; u < kVectors; u += 2) {
+      float f[2 * E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = to_float(x[u].at[e]), f[E + e] = to_float(x[u + 1].at[e]);
+      r.add(f, c);
+    }
   }
-  const float top = block_max(m, part);
-  s = block_sum(m == -INFINITY ? s : s * exp2_fast((m - top) * c), part);
-  if (threadIdx.x == 0 && stats) stats[row] = make_float2(top, s);
-  float t_top, t_total;
-  const bool some = load_teacher(ids, wide, teacher, row * k, k, V, c, id, e, part, t_top, t_total);
-  // log p - log q = (t - t_top) / tau - log t_total - (z - top) / tau + log s
-  const float apart = logf(s) - logf(t_total);
-  float sum = 0.f;
-  for (int j = threadIdx.x; j < k; j += kThreads)
-    if (id[j] >= 0 && e[j] != 0.f)
-      sum += e[j] * (((teacher[row * k + j] - t_top) - (to_float(z[id[j]]) - top)) / tau + apart);
-  sum = block_sum(sum, part);
-  if (threadIdx.x == 0) loss[row] = some ? sum / t_total * tau * tau : 0.f;
+  for (; v < end; v += NT) {
+    vec x;
+    x.raw = __ldg(words + v);
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = to_float(x.at[e]);
+    r.add(f, c);
+  }
+  float top = row_reduce<NT>(r.top, maximum(), part);
+  float total = row_reduce<NT>(r.under(top, c), sum(), part);
+  if (CL > 1) {   // the blocks' parts, in the order of their ranks
+    if (threadIdx.x == 0) {
+      uint32_t to;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&from_rank[rank])));
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(top), "f"(total) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0) return;
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < CL; ++i) most = fmaxf(most, from_rank[i].x);
+    total = 0.f;
+#pragma unroll
+    for (int i = 0; i < CL; ++i) {
+      running other;
+      other.top = from_rank[i].x, other.total = from_rank[i].y;
+      total += other.under(most, c);
+    }
+    top = most;
+  }
+  if (tid == 0 && stats) stats[row] = make_float2(top, total);
+  row_sync<NT>();
+  float t_top = -INFINITY;
+  for (int j = tid; j < k; j += NT) t_top = fmaxf(t_top, of_teacher[slot][j]);
+  // (no entry but one of -infinity does not count; one that is no number leaves the maximum alone)
+  bool some = false;
+  for (int j = tid; j < k; j += NT) some = some || of_teacher[slot][j] != -INFINITY;
+  some = row_any<NT>(some);
+  t_top = row_reduce<NT>(t_top, maximum(), part);
+  float t_total = 0.f;
+  for (int j = tid; j < k; j += NT) t_total += of_teacher[slot][j] == -INFINITY ? 0.f : exp2_fast((of_teacher[slot][j] - t_top) * c);
+  t_total = row_reduce<NT>(t_total, sum(), part);
+  // log p - log q = (t - t_top) / tau - log t_total - (z - top) / tau + log total
+  const float apart = logf(total) - logf(t_total);
+  float value = 0.f;
+  for (int j = tid; j < k; j += NT) {
+    const float t = of_teacher[slot][j], e = t == -INFINITY ? 0.f : exp2_fast((t - t_top) * c);
+    if (e != 0.f) value += e * (((t - t_top) - (of_student[slot][j] - top)) / tau + apart);
+  }
+  value = row_reduce<NT>(value, sum(), part);
+  if (tid == 0) loss[row] = some ? value / t_total * tau * tau : 0.f;
 }
 
-template <typename T>
+// One read and one write of the row; the columns that the teacher names are written again by the first of their entries.
+// slices: blocks to a row where rows are few.  The last rows come first: the forward pass left them in the L2 cache.
+template <typename T, int NT>
 __global__ void __launch_bounds__(kThreads)
-distill_backward_kernel(int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
+distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
                         const float* __restrict__ teacher, float tau, const float2* __restrict__ stats,
-                        const float* __restrict__ dloss, int64_t dloss_stride, T* __restrict__ dlogits) {
-  __shared__ int id[kMaxEntries];
-  __shared__ float e[kMaxEntries], part[kWarps];
-  const int64_t row = blockIdx.x;
+                        const float* __restrict__ dloss, int64_t dloss_stride, T* __restrict__ dlogits, int slices) {
+  typedef dense_vec<T, 16> vec;
+  constexpr int E = vec::kCount;
+  constexpr int kRows = kThreads / NT, kEntries = NT == 32 ? kMaxEntriesWarp : kMaxEntries;
+  __shared__ int id_of[kRows][kEntries];
+  __shared__ float p_of[kRows][kEntries], part[kThreads / 32];
+  const int tid = threadIdx.x & (NT - 1), slot = NT == 32 ? threadIdx.x >> 5 : 0;
+  const int64_t back = NT == 32 ? (int64_t)blockIdx.x * kRows + slot : blockIdx.x / slices;
+  const int slice = NT == 32 ? 0 : (int)(blockIdx.x - back * slices);
+  if (back >= rows) return;             // whole warps, and none of them in front of a barrier of the block
+  const int64_t row = rows - 1 - back;
   const T* z = logits + row * ld;
   T* dz = dlogits + row * V;
+  int* id = id_of[slot];
+  float* p = p_of[slot];
   const float c = kLog2e / tau;
-  float t_top, t_total;
-  const bool some = load_teacher(ids, wide, teacher, row * k, k, V, c, id, e, part, t_top, t_total);
-  if (!some) {
-    for (int v = threadIdx.x; v < V; v += kThreads) dz[v] = from_float<T>(0.f);
-    return;
-  }
   const float2 st = stats[row];
   const float g = dloss[row * dloss_stride] * tau, q = 1.f / st.y;
-  for (int v = threadIdx.x; v < V; v += kThreads)
-    dz[v] = from_float<T>(g * (exp2_fast((to_float(z[v]) - st.x) * c) * q));
-  __syncthreads();
-  // the columns that the teacher names once more, each by the first of its entries
-  const float per = 1.f / t_total;
-  for (int j = threadIdx.x; j < k; j += kThreads) {
+  float t_top = -INFINITY;
+  bool some = false;
+  for (int j = tid; j < k; j += NT) {
+    const float t = teacher[row * k + j];
+    const int i = t == -INFINITY ? -1 : load_id(ids, wide, row * k + j, V);
+    id[j] = i, p[j] = t;
+    if (i >= 0) some = true, t_top = fmaxf(t_top, t);
+  }
+  some = row_any<NT>(some);
+  t_top = row_reduce<NT>(t_top, maximum(), part);
+  float t_total = 0.f;
+  for (int j = tid; j < k; j += NT) {
+    const float e = id[j] >= 0 ? exp2_fast((p[j] - t_top) * c) : 0.f;
+    p[j] = e;
+    t_total += e;
+  }
+  const float per = 1.f / row_reduce<NT>(t_total, sum(), part);
+  auto value = [&](float x) { return some ? g * (exp2_fast((x - st.x) * c) * q) : 0.f; };
+  const row_parts<T> at(z, V), to(dz, V);
+  const int body = at.head == to.head ? at.vectors : 0;
+  const int begin = (int)((int64_t)body * slice / slices), end = (int)((int64_t)body * (slice + 1) / slices);
+  if (at.head == to.head) {
+    if (slice == 0)
+      for (int v = tid; v < at.head; v += NT) dz[v] = from_float<T>(value(to_float(z[v])));
+    if (slice == slices - 1)
+      for (int v = at.tail + tid; v < V; v += NT) dz[v] = from_float<T>(value(to_float(z[v])));
+  } else {   // rows of the two that begin differently: element by element
+    for (int64_t v = (int64_t)V * slice / slices + tid; v < (int64_t)V * (slice + 1) / slices; v += NT)
+      dz[v] = from_float<T>(value(to_float(z[v])));
+  }
+  const uint4* words = reinterpret_cast<const uint4*>(z + at.head);
+  uint4* out = reinterpret_cast<uint4*>(dz + at.head);
+  for (int v0 = begin + tid; v0 < end; v0 += kVectors * NT) {
+    vec x[kVectors];
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u)
+      if (v0 + u * NT < end) x[u].raw = __ldg(words + v0 + u * NT);
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u)
+      if (v0 + u * NT < end) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u].at[e] = from_float<T>(value(to_float(x[u].at[e])));
+        out[v0 + u * NT] = x[u].raw;
+      }
+  }
+  row_sync<NT>();
+  if (!some) return;
+  // the columns of this slice
+  const int64_t lo = at.head != to.head ? (int64_t)V * slice / slices : (slice == 0 ? 0 : at.head + (int64_t)begin * E);
+  const int64_t hi = at.head != to.head ? (int64_t)V * (slice + 1) / slices : (slice == slices - 1 ? V : at.head + (int64_t)end * E);
+  for (int j = tid; j < k; j += NT) {
     const int v = id[j];
-    if (v < 0) continue;
-    float p = 0.f;
+    if (v < lo || v >= hi || v < 0) continue;
+    float share = 0.f;
     bool first = true;
     for (int i = 0; i < k; ++i)
       if (id[i] == v) {
         first = first && i >= j;
-        p += e[i];
+        share += p[i];
       }
-    if (first) dz[v] = from_float<T>(g * (exp2_fast((to_float(z[v]) - st.x) * c) * q - p * per));
+    if (first) dz[v] = from_float<T>(g * (exp2_fast((to_float(z[v]) - st.x) * c) * q - share * per));
   }
+}
+
+// A warp to a row where rows are short and many enough to fill the warps; blocks to a row where there are few rows, each with
+// at least 16 KB of it.
+struct distill_shape {
+  bool warp;
+  int parts;
+};
+distill_shape choose_distill(const hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int size) {
+  distill_shape sh = {V * size <= 4096 && k <= kMaxEntriesWarp, 1};
+  while (!sh.warp && sh.parts < 8 && T * sh.parts < 2 * ctx->sm_count && V * size >= (int64_t)sh.parts * 32768) sh.parts *= 2;
+  return sh;
+}
+
+template <typename T, int CL>
+cudaError_t launch_cluster(int64_t rows, int V, int k, const void* logits, int64_t ld, const void* ids, int wide, const float* teacher,
+                           float tau, float* loss, float* stats, cudaStream_t s) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CL, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((unsigned)(rows * CL)), c.blockDim = dim3(kThreads), c.stream = s, c.attrs = &attr, c.numAttrs = CL > 1;
+  return cudaLaunchKernelEx(&c, distill_forward_kernel<T, kThreads, CL>, rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, loss,
+                            (float2*)stats);
+}
+
+template <typename T>
+cudaError_t launch_forward(hpspmm_ctx* ctx, int64_t rows, int V, int k, const void* logits, int64_t ld, const void* ids, int wide,
+                           const float* teacher, float tau, float* loss, float* stats, cudaStream_t s) {
+  const distill_shape sh = choose_distill(ctx, rows, V, k, (int)sizeof(T));
+  if (sh.warp) {
+    distill_forward_kernel<T, 32, 1><<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher,
+                                                                                    tau, loss, (float2*)stats);
+    return cudaSuccess;
+  }
+  if (sh.parts == 8) return launch_cluster<T, 8>(rows, V, k, logits, ld, ids, wide, teacher, tau, loss, stats, s);
+  if (sh.parts == 4) return launch_cluster<T, 4>(rows, V, k, logits, ld, ids, wide, teacher, tau, loss, stats, s);
+  if (sh.parts == 2) return launch_cluster<T, 2>(rows, V, k, logits, ld, ids, wide, teacher, tau, loss, stats, s);
+  return launch_cluster<T, 1>(rows, V, k, logits, ld, ids, wide, teacher, tau, loss, stats, s);
+}
+
+template <typename T>
+void launch_backward(hpspmm_ctx* ctx, int64_t rows, int V, int k, const void* logits, int64_t ld, const void* ids, int wide,
+                     const float* teacher, float tau, const float* stats, const float* dloss, int64_t stride, void* dlogits,
+                     cudaStream_t s) {
+  const distill_shape sh = choose_distill(ctx, rows, V, k, (int)sizeof(T));
+  if (sh.warp)
+    distill_backward_kernel<T, 32><<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(
+        rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, (const float2*)stats, dloss, stride, (T*)dlogits, 1);
+  else
+    distill_backward_kernel<T, kThreads><<<(unsigned)(rows * sh.parts), kThreads, 0, s>>>(
+        rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, (const float2*)stats, dloss, stride, (T*)dlogits, sh.parts);
 }
 
 int check_distill(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int32_t type, int64_t ld, int32_t id_bytes, float tau) {
@@ -181,15 +363,14 @@ int hpspmm_topk_distill_forward(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   const int wide = id_bytes == 8;
+  cudaError_t e;
   if (type == HPSPMM_TYPE_F32)
-    distill_forward_kernel<<<(unsigned)T, kThreads, 0, s>>>((int)V, (int)k, (const float*)logits, ld_logits, ids, wide,
-                                                            teacher_logits, temperature, loss, (float2*)stats);
+    e = launch_forward<float>(ctx, T, (int)V, (int)k, logits, ld_logits, ids, wide, teacher_logits, temperature, loss, stats, s);
   else if (type == HPSPMM_TYPE_F16)
-    distill_forward_kernel<<<(unsigned)T, kThreads, 0, s>>>((int)V, (int)k, (const __half*)logits, ld_logits, ids, wide,
-                                                            teacher_logits, temperature, loss, (float2*)stats);
+    e = launch_forward<__half>(ctx, T, (int)V, (int)k, logits, ld_logits, ids, wide, teacher_logits, temperature, loss, stats, s);
   else
-    distill_forward_kernel<<<(unsigned)T, kThreads, 0, s>>>((int)V, (int)k, (const __nv_bfloat16*)logits, ld_logits, ids, wide,
-                                                            teacher_logits, temperature, loss, (float2*)stats);
+    e = launch_forward<__nv_bfloat16>(ctx, T, (int)V, (int)k, logits, ld_logits, ids, wide, teacher_logits, temperature, loss, stats, s);
+  HPSPMM_CUDA_TRY(ctx, e);
   ctx->launches++;
   HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
   return HPSPMM_OK;
@@ -209,17 +390,14 @@ int hpspmm_topk_distill_backward(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t 
   cudaStream_t s = (cudaStream_t)stream;
   const int wide = id_bytes == 8;
   if (type == HPSPMM_TYPE_F32)
-    distill_backward_kernel<<<(unsigned)T, kThreads, 0, s>>>((int)V, (int)k, (const float*)logits, ld_logits, ids, wide,
-                                                             teacher_logits, temperature, (const float2*)stats, dloss,
-                                                             dloss_stride, (float*)dlogits);
+    launch_backward<float>(ctx, T, (int)V, (int)k, logits, ld_logits, ids, wide, teacher_logits, temperature, stats, dloss, dloss_stride,
+                           dlogits, s);
   else if (type == HPSPMM_TYPE_F16)
-    distill_backward_kernel<<<(unsigned)T, kThreads, 0, s>>>((int)V, (int)k, (const __half*)logits, ld_logits, ids, wide,
-                                                             teacher_logits, temperature, (const float2*)stats, dloss,
-                                                             dloss_stride, (__half*)dlogits);
+    launch_backward<__half>(ctx, T, (int)V, (int)k, logits, ld_logits, ids, wide, teacher_logits, temperature, stats, dloss, dloss_stride,
+                            dlogits, s);
   else
-    distill_backward_kernel<<<(unsigned)T, kThreads, 0, s>>>((int)V, (int)k, (const __nv_bfloat16*)logits, ld_logits, ids, wide,
-                                                             teacher_logits, temperature, (const float2*)stats, dloss,
-                                                             dloss_stride, (__nv_bfloat16*)dlogits);
+    launch_backward<__nv_bfloat16>(ctx, T, (int)V, (int)k, logits, ld_logits, ids, wide, teacher_logits, temperature, stats, dloss,
+                                   dloss_stride, dlogits, s);
   ctx->launches++;
   HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
   return HPSPMM_OK;
