@@ -14,28 +14,33 @@ using namespace hpspmm;
 
 constexpr int kThreads = 256;
 
-// One thread to a vector of the output.
-template <typename T, int BYTES>
+// A group of W lanes to a piece of 4 W vectors of one row, all of them in flight at once.
+template <typename T, int BYTES, int W>
 __global__ void __launch_bounds__(kThreads)
-lookup_kernel(int64_t total, int per_row, int N, const void* __restrict__ ids, int wide, const T* __restrict__ table,
-              int64_t ld, float scale, T* __restrict__ out) {
+lookup_kernel(int64_t groups, int pieces, int per_row, int N, const void* ids, int wide, const T* table, int64_t ld, float scale,
+              T* __restrict__ out) {
   typedef dense_vec<T, BYTES> vec;
-  const int64_t stride = (int64_t)gridDim.x * kThreads;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += stride) {
-    const int64_t t = i / per_row;
-    const int c = (int)(i - t * per_row) * vec::kCount;
-    const int id = load_id(ids, wide, t, N);
-    vec v;
-    if (id >= 0) {
-      v.raw = *reinterpret_cast<const decltype(v.raw)*>(table + (int64_t)id * ld + c);
+  chain_grid();
+  const int64_t group = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / W;
+  if (group >= groups) return;
+  const int64_t t = pieces == 1 ? group : group / pieces;
+  const int first = (int)(group - t * pieces) * 4 * W + (threadIdx.x & (W - 1));
+  const int id = load_id(ids, wide, t, N);
+  const T* src = table + (int64_t)id * ld;
+  T* to = out + t * ((int64_t)per_row * vec::kCount);
+  vec v[4];
+  if (id >= 0) {
 #pragma unroll
-      for (int e = 0; e < vec::kCount; ++e) v.at[e] = from_float<T>(scale * to_float(v.at[e]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < vec::kCount; ++e) v.at[e] = from_float<T>(0.f);
-    }
-    reinterpret_cast<decltype(v.raw)*>(out)[i] = v.raw;
+    for (int u = 0; u < 4; ++u)
+      if (first + u * W < per_row) v[u].raw = *reinterpret_cast<const decltype(v[u].raw)*>(src + (int64_t)(first + u * W) * vec::kCount);
   }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (first + u * W < per_row) {
+#pragma unroll
+      for (int e = 0; e < vec::kCount; ++e) v[u].at[e] = from_float<T>(id >= 0 ? scale * to_float(v[u].at[e]) : 0.f);
+      reinterpret_cast<decltype(v[u].raw)*>(to)[first + u * W] = v[u].raw;
+    }
 }
 
 // ---- positions sorted by id ----------------------------------------------------------------------------------------
@@ -77,47 +82,52 @@ rank_kernel(int T, int N, const void* ids, int wide, int* key_out, int* pos_out)
   }
 }
 
-// Radix sort by digits of up to 9 bits, for more positions.  Block b of each pass has the positions [b * chunk, ...).
-constexpr int kDigits = 512;
-constexpr int kSortThreads = 512;
+// Radix sort by digits of up to 10 bits, for more positions.  Block b of each pass has the positions [b * chunk, ...).
+// Every block adds up the counts of all blocks itself, which costs blocks^2 * digits loads, so the blocks are few and
+// large: with 148 of 2048 positions a pass over 262,144 positions took 13.2 us, with 64 of 4096 it takes 17.4 us with 10-bit digits, two passes instead of three.
+constexpr int kMaxDigitBits = 10;
+constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortBlocks = 148;      // at most
-constexpr int kSortChunk = 2048;      // positions to a block, at least
 
 // Counts of the first digit; the tables of the later ones, which the passes in front of them fill, are cleared.
 __global__ void __launch_bounds__(kSortThreads)
-digit_count_kernel(int64_t T, int N, const void* ids, int wide, int64_t chunk, int digit_mask, int passes, int* tables) {
-  __shared__ int count[kDigits];
+digit_count_kernel(int64_t T, int N, const void* ids, int wide, int64_t chunk, int digits, int passes, int* tables) {
+  __shared__ int count[1 << kMaxDigitBits];
   chain_grid();
   count[threadIdx.x] = 0;
   __syncthreads();
   const int64_t end = min(T, (blockIdx.x + 1) * chunk);
   for (int64_t t = blockIdx.x * chunk + threadIdx.x; t < end; t += kSortThreads)
-    atomicAdd(count + (key_of(ids, wide, t, N) & digit_mask), 1);
+    atomicAdd(count + (key_of(ids, wide, t, N) & (digits - 1)), 1);
   __syncthreads();
-  tables[blockIdx.x * kDigits + threadIdx.x] = count[threadIdx.x];
-  for (int p = 1; p < passes; ++p) tables[((int64_t)p * gridDim.x + blockIdx.x) * kDigits + threadIdx.x] = 0;
+  if (threadIdx.x < digits) {
+    tables[blockIdx.x * digits + threadIdx.x] = count[threadIdx.x];
+    for (int p = 1; p < passes; ++p) tables[((int64_t)p * gridDim.x + blockIdx.x) * digits + threadIdx.x] = 0;
+  }
 }
 
 // One pass: positions to their places by one digit, in order within a digit.  keys_in is null in the first pass, which
 // reads the ids.  next: the counts of the next digit by block of the new order, or null in the last pass.
 __global__ void __launch_bounds__(kSortThreads)
 digit_place_kernel(int64_t T, int N, const void* ids, int wide, const int* keys_in, const int* pos_in, int64_t chunk, int shift,
-                   int digit_mask, int next_shift, const int* table, int* next, int* keys_out, int* pos_out) {
-  __shared__ int place[kSortWarps][kDigits];
-  __shared__ int of_digit[kDigits], of_digit_before[kDigits];
+                   int bits, const int* table, int* next, int* keys_out, int* pos_out) {
+  extern __shared__ int places[];      // [warp][digit]
+  __shared__ int of_digit[1 << kMaxDigitBits], of_digit_before[1 << kMaxDigitBits];
   __shared__ int warp_sum[kSortWarps];
   chain_grid();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int digits = 1 << bits, mask = digits - 1;
+  int* place = places + warp * digits;
   auto key_at = [&](int64_t t) { return keys_in ? keys_in[t] : key_of(ids, wide, t, N); };
   of_digit[threadIdx.x] = of_digit_before[threadIdx.x] = 0;
+  for (int d = lane; d < digits; d += 32) place[d] = 0;
   __syncthreads();
   {   // of every digit: how many there are, and how many in the blocks in front of this one
-    const int quad = threadIdx.x & 127, group = threadIdx.x >> 7;
+    const int quads = digits / 4, quad = threadIdx.x & (quads - 1), group = threadIdx.x / quads, groups = kSortThreads / quads;
     int4 all = make_int4(0, 0, 0, 0), before = all;
-#pragma unroll 4
-    for (int b = group; b < gridDim.x; b += 4) {
-      const int4 c = reinterpret_cast<const int4*>(table)[b * (kDigits / 4) + quad];
+#pragma unroll 8
+    for (int b = group; b < gridDim.x; b += groups) {
+      const int4 c = reinterpret_cast<const int4*>(table)[b * quads + quad];
       all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
       if (b < blockIdx.x) before.x += c.x, before.y += c.y, before.z += c.z, before.w += c.w;
     }
@@ -126,15 +136,13 @@ digit_place_kernel(int64_t T, int N, const void* ids, int wide, const int* keys_
     atomicAdd(to_before, before.x), atomicAdd(to_before + 1, before.y), atomicAdd(to_before + 2, before.z), atomicAdd(to_before + 3, before.w);
   }
   const int64_t begin = blockIdx.x * chunk, end = min(T, begin + chunk);
-  const int64_t sub = (chunk / kSortWarps + 31) / 32 * 32;
+  const int64_t sub = chunk / kSortWarps;
   const int64_t from = min(end, begin + warp * sub), to = min(end, from + sub);
-  for (int d = lane; d < kDigits; d += 32) place[warp][d] = 0;
-  __syncwarp();
-  for (int64_t t = from + lane; t < to; t += 32) atomicAdd(&place[warp][key_at(t) >> shift & digit_mask], 1);
+  for (int64_t t = from + lane; t < to; t += 32) atomicAdd(place + (key_at(t) >> shift & mask), 1);
   __syncthreads();
   {   // places of every warp's digits
     const int d = threadIdx.x;
-    const int all = of_digit[d], before = of_digit_before[d];
+    const int all = d < digits ? of_digit[d] : 0;
     int sum = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -143,13 +151,15 @@ digit_place_kernel(int64_t T, int N, const void* ids, int wide, const int* keys_
     }
     if (lane == 31) warp_sum[warp] = sum;
     __syncthreads();
-    int at = sum - all + before;
-    for (int w = 0; w < warp; ++w) at += warp_sum[w];
-#pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int n = place[w][d];
-      place[w][d] = at;
-      at += n;
+    if (d < digits) {
+      int at = sum - all + of_digit_before[d];
+      for (int w = 0; w < warp; ++w) at += warp_sum[w];
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const int n = places[w * digits + d];
+        places[w * digits + d] = at;
+        at += n;
+      }
     }
   }
   __syncthreads();
@@ -157,17 +167,17 @@ digit_place_kernel(int64_t T, int N, const void* ids, int wide, const int* keys_
     const int64_t t = t0 + lane;
     const bool have = t < to;
     const int key = have ? key_at(t) : 0;
-    const int d = have ? key >> shift & digit_mask : kDigits;
+    const int d = have ? key >> shift & mask : digits;
     const unsigned same = __match_any_sync(0xffffffffu, d);
     const int before = __popc(same & ((1u << lane) - 1));
     int at = 0;
-    if (have) at = place[warp][d] + before;
+    if (have) at = place[d] + before;
     __syncwarp();
     if (have) {
-      if (before == 0) place[warp][d] = at + __popc(same);
+      if (before == 0) place[d] = at + __popc(same);
       keys_out[at] = key;
       pos_out[at] = pos_in ? pos_in[t] : (int)t;
-      if (next) atomicAdd(next + at / chunk * kDigits + (key >> next_shift & digit_mask), 1);
+      if (next) atomicAdd(next + (int64_t)((unsigned)at / (unsigned)chunk) * digits + (key >> (shift + bits) & mask), 1);
     }
     __syncwarp();
   }
@@ -300,18 +310,21 @@ sum_parts_kernel(int n, int N, int K, int64_t parts, int slabs, int length, cons
   if (!last_is_row) to_split(1);
 }
 
-// Rows that lie in several parts.  A block looks at 8 parts, one to a warp: a row that began earlier and ends in the part is
-// the sum of the pieces before it and its own; many pieces are shared by the block's warps.
+// Rows that lie in several parts.  A block has 8 parts, one to a warp, and 128 columns: a row that began earlier and ends in
+// the part is the sum of the pieces before it and its own.  The warps share the pieces of rows that have many.
+constexpr int kJoinColumns = 128;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 join_parts_kernel(int N, int K, int64_t parts, const int2* info, const float* split, float scale, T* __restrict__ dtable) {
   constexpr int kWarps = kThreads / 32;
   __shared__ int64_t first_of[kWarps];
   __shared__ int row_of[kWarps];
-  __shared__ float sums[kWarps][32];
+  __shared__ float sums[kWarps][kJoinColumns];
   chain_grid();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t part = (int64_t)blockIdx.x * kWarps + warp;
+  const int col = blockIdx.y * kJoinColumns + lane;
   int row = -1;
   int64_t first = 0;
   if (part < parts) {
@@ -330,39 +343,46 @@ join_parts_kernel(int N, int K, int64_t parts, const int2* info, const float* sp
       first = info[lo].y ? lo - 1 : lo;   // (open: its beginning is the part in front)
     }
   }
-  if (lane == 0) row_of[warp] = row, first_of[warp] = first;
+  // columns lane, lane + 32, ... of pieces [b, e)
+  auto add = [&](int64_t b, int64_t e, float (&sum)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = 0.f;
+#pragma unroll 4
+    for (int64_t s = b; s < e; ++s) {
+      const float* p = split + (2 * s + 1) * K + col;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (col + 32 * i < K) sum[i] += p[32 * i];
+    }
+  };
+  const bool many = row >= 0 && part - first > 4 * kWarps;
+  if (row >= 0 && !many) {
+    float sum[4];
+    add(first, part, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + 32 * i < K)
+        dtable[(int64_t)row * K + col + 32 * i] = from_float<T>(scale * (sum[i] + split[2 * part * K + col + 32 * i]));
+  }
+  if (lane == 0) row_of[warp] = many ? row : -1, first_of[warp] = first;
   __syncthreads();
   for (int w = 0; w < kWarps; ++w) {
     const int r = row_of[w];
     if (r < 0) continue;
-    const int64_t f = first_of[w], mine = (int64_t)blockIdx.x * kWarps + w, pieces = mine - f;
-    T* to = dtable + (int64_t)r * K;
-    if (pieces <= 2 * kWarps) {
-      for (int c = threadIdx.x; c < K; c += kThreads) {
-        float sum = 0.f;
-        for (int64_t s = f; s < mine; ++s) sum += split[(2 * s + 1) * K + c];
-        to[c] = from_float<T>(scale * (sum + split[2 * mine * K + c]));
-      }
-    } else {
-      const int64_t b = f + pieces * warp / kWarps, e = f + pieces * (warp + 1) / kWarps;
-      for (int c0 = 0; c0 < K; c0 += 32) {
-        const int c = c0 + lane;
-        float sum = 0.f;
-        if (c < K) {
-#pragma unroll 8
-          for (int64_t s = b; s < e; ++s) sum += split[(2 * s + 1) * K + c];
-        }
-        sums[warp][lane] = sum;
-        __syncthreads();
-        if (warp == 0 && c < K) {
-          sum = sums[0][lane];
+    const int64_t f = first_of[w], own = (int64_t)blockIdx.x * kWarps + w, pieces = own - f;
+    float sum[4];
+    add(f + pieces * warp / kWarps, f + pieces * (warp + 1) / kWarps, sum);
 #pragma unroll
-          for (int i = 1; i < kWarps; ++i) sum += sums[i][lane];
-          to[c] = from_float<T>(scale * (sum + split[2 * mine * K + c]));
-        }
-        __syncthreads();
-      }
+    for (int i = 0; i < 4; ++i) sums[warp][lane + 32 * i] = sum[i];
+    __syncthreads();
+    const int c = blockIdx.y * kJoinColumns + threadIdx.x;
+    if (threadIdx.x < kJoinColumns && c < K) {
+      float all = sums[0][threadIdx.x];
+#pragma unroll
+      for (int i = 1; i < kWarps; ++i) all += sums[i][threadIdx.x];
+      dtable[(int64_t)r * K + c] = from_float<T>(scale * (all + split[2 * own * K + c]));
     }
+    __syncthreads();
   }
 }
 
@@ -383,11 +403,12 @@ backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
   backward_plan p = {};
   while (p.bits < 31 && ((int64_t)1 << p.bits) <= N) ++p.bits;
   if (T > kRankMost) {
-    p.passes = (p.bits + 8) / 9;
-    p.bits = (p.bits + p.passes - 1) / p.passes;
+    p.passes = (p.bits + kMaxDigitBits - 1) / kMaxDigitBits;
+    p.bits = std::max(5, (p.bits + p.passes - 1) / p.passes);
   }
-  p.chunk = std::max<int64_t>(kSortChunk, (T + kSortBlocks - 1) / kSortBlocks);
-  p.chunk = (p.chunk + kSortThreads - 1) / kSortThreads * kSortThreads;
+  p.chunk = (T + 63) / 64;
+  if (T > 1 << 20) p.chunk = (T + 147) / 148;
+  p.chunk = std::max<int64_t>(1, (p.chunk + kSortThreads - 1) / kSortThreads) * kSortThreads;
   p.blocks = (int)((T + p.chunk - 1) / p.chunk);
   p.length = (T + N) * ((K + 255) / 256) < 148 * 32 * 64 ? 16 : 64;
   p.parts = (T + N + p.length - 1) / p.length;
@@ -395,7 +416,7 @@ backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
   p.keys = 0;
   p.pos = p.keys + b_t * (p.passes > 1 ? 2 : 1);
   p.tables = p.pos + b_t * (p.passes > 1 ? 2 : 1);
-  p.info = p.tables + align_up((size_t)p.passes * p.blocks * kDigits * 4, 256);
+  p.info = p.tables + align_up((size_t)p.passes * p.blocks * ((size_t)4 << p.bits), 256);
   p.split = p.info + align_up((size_t)p.parts * sizeof(int2), 256);
   p.bytes = p.split + (size_t)p.parts * 2 * K * 4;
   return p;
@@ -414,8 +435,9 @@ void launch_sort(hpspmm_ctx* ctx, const backward_plan& p, int64_t T, int64_t N, 
     return;
   }
   int* tables = (int*)(space + p.tables);
-  const int mask = (1 << p.bits) - 1;
-  hpspmm_launch(digit_count_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, T, (int)N, ids, wide, p.chunk, mask, p.passes, tables);
+  const int digits = 1 << p.bits, smem = kSortWarps * digits * 4;
+  cudaFuncSetAttribute(digit_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);   // (a refusal shows at the launch)
+  hpspmm_launch(digit_count_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, T, (int)N, ids, wide, p.chunk, digits, p.passes, tables);
   ctx->launches++;
   for (int i = 0; i < p.passes; ++i) {
     // the last pass writes the first buffers
@@ -423,9 +445,9 @@ void launch_sort(hpspmm_ctx* ctx, const backward_plan& p, int64_t T, int64_t N, 
     int* to_p = (p.passes - 1 - i) % 2 ? (int*)((char*)at + b_t) : at;
     const int* from_k = i == 0 ? nullptr : (to_k == k ? (int*)((char*)k + b_t) : k);
     const int* from_p = i == 0 ? nullptr : (to_p == at ? (int*)((char*)at + b_t) : at);
-    const int64_t table = (int64_t)p.blocks * kDigits;
-    hpspmm_launch(digit_place_kernel, dim3(p.blocks), dim3(kSortThreads), 0, s, T, (int)N, ids, wide, from_k, from_p, p.chunk, i * p.bits,
-                  mask, (i + 1) * p.bits, tables + i * table, i + 1 < p.passes ? tables + (i + 1) * table : nullptr, to_k, to_p);
+    const int64_t table = (int64_t)p.blocks * digits;
+    hpspmm_launch(digit_place_kernel, dim3(p.blocks), dim3(kSortThreads), smem, s, T, (int)N, ids, wide, from_k, from_p, p.chunk, i * p.bits,
+                  p.bits, tables + i * table, i + 1 < p.passes ? tables + (i + 1) * table : nullptr, to_k, to_p);
     ctx->launches++;
   }
 }
@@ -438,8 +460,8 @@ void launch_sums(hpspmm_ctx* ctx, const backward_plan& p, int64_t n, int64_t N, 
   hpspmm_launch(sum_parts_kernel<T, BYTES, R, W>, dim3((unsigned)((lanes + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, (int)n, (int)N,
                 (int)K, p.parts, (int)slabs, p.length, keys, pos, (const T*)dout, ld, scale, (T*)dtable, (int2*)(space + p.info),
                 (float*)(space + p.split));
-  hpspmm_launch(join_parts_kernel<T>, dim3((unsigned)((p.parts + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads), 0, s, (int)N, (int)K,
-                p.parts, (const int2*)(space + p.info), (const float*)(space + p.split), scale, (T*)dtable);
+  hpspmm_launch(join_parts_kernel<T>, dim3((unsigned)((p.parts + kThreads / 32 - 1) / (kThreads / 32)), (unsigned)((K + kJoinColumns - 1) / kJoinColumns)),
+                dim3(kThreads), 0, s, (int)N, (int)K, p.parts, (const int2*)(space + p.info), (const float*)(space + p.split), scale, (T*)dtable);
   ctx->launches += 2;
 }
 
@@ -465,28 +487,34 @@ void launch_sums_of(hpspmm_ctx* ctx, const backward_plan& p, int64_t n, int64_t 
 }
 
 template <typename T, int BYTES>
-void launch_lookup(hpspmm_ctx* ctx, int64_t T_, int64_t N, int64_t K, const void* ids, int wide, const void* table,
-                   int64_t ld, float scale, void* out, cudaStream_t s) {
+void launch_lookup(int64_t T_, int64_t N, int64_t K, const void* ids, int wide, const void* table, int64_t ld, float scale, void* out,
+                   cudaStream_t s) {
   const int per_row = (int)(K * (int64_t)sizeof(T) / BYTES);
-  const int64_t total = T_ * per_row;
-  const int64_t blocks = std::min<int64_t>((total + kThreads - 1) / kThreads, (int64_t)ctx->sm_count * 32);
-  lookup_kernel<T, BYTES><<<(unsigned)blocks, kThreads, 0, s>>>(total, per_row, (int)N, ids, wide, (const T*)table, ld,
-                                                                scale, (T*)out);
+  // rows of up to 32 vectors: 8 lanes with up to four each, so that as much is in flight as with wide rows
+  const int W = per_row <= 32 ? 8 : 32;
+  const int64_t pieces = (per_row + 4 * W - 1) / (4 * W), groups = T_ * pieces;
+  const dim3 grid((unsigned)((groups * W + kThreads - 1) / kThreads));
+  if (W == 8)
+    hpspmm_launch(lookup_kernel<T, BYTES, 8>, grid, dim3(kThreads), 0, s, groups, (int)pieces, per_row, (int)N, ids, wide, (const T*)table, ld,
+                  scale, (T*)out);
+  else
+    hpspmm_launch(lookup_kernel<T, BYTES, 32>, grid, dim3(kThreads), 0, s, groups, (int)pieces, per_row, (int)N, ids, wide, (const T*)table,
+                  ld, scale, (T*)out);
 }
 
 template <typename T>
-void launch_lookup_of(hpspmm_ctx* ctx, int64_t T_, int64_t N, int64_t K, const void* ids, int wide, const void* table,
+void launch_lookup_of(int64_t T_, int64_t N, int64_t K, const void* ids, int wide, const void* table,
                       int64_t ld, float scale, void* out, cudaStream_t s) {
   const int bytes = dense_vector_bytes((uintptr_t)table | (uintptr_t)out | (uintptr_t)(K * (int64_t)sizeof(T)) |
                                            (uintptr_t)(ld * (int64_t)sizeof(T)), (int)sizeof(T));
   if (bytes == 16)
-    launch_lookup<T, 16>(ctx, T_, N, K, ids, wide, table, ld, scale, out, s);
+    launch_lookup<T, 16>(T_, N, K, ids, wide, table, ld, scale, out, s);
   else if (bytes == 8)
-    launch_lookup<T, 8>(ctx, T_, N, K, ids, wide, table, ld, scale, out, s);
+    launch_lookup<T, 8>(T_, N, K, ids, wide, table, ld, scale, out, s);
   else if (bytes == 4 || sizeof(T) == 4)
-    launch_lookup<T, 4>(ctx, T_, N, K, ids, wide, table, ld, scale, out, s);
+    launch_lookup<T, 4>(T_, N, K, ids, wide, table, ld, scale, out, s);
   else
-    launch_lookup<T, sizeof(T)>(ctx, T_, N, K, ids, wide, table, ld, scale, out, s);
+    launch_lookup<T, sizeof(T)>(T_, N, K, ids, wide, table, ld, scale, out, s);
 }
 
 int check_embedding(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, int32_t type, int32_t id_bytes, int64_t ld) {
@@ -513,14 +541,16 @@ int hpspmm_embedding_forward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, i
   HPSPMM_REQUIRE(ctx, ld_table >= K, "row stride below the number of columns");
   if (T == 0 || K == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, ids && out && (table || N == 0), "null pointer");
+  // a group of lanes moves at least four elements of each of its lanes, or a row of up to 32 vectors
+  if (T > ((int64_t)1 << 33) / ((K + 127) / 128)) return hpspmm_unsupported(ctx, "more than 2^31 - 1 blocks");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   if (type == HPSPMM_TYPE_F32)
-    launch_lookup_of<float>(ctx, T, N, K, ids, id_bytes == 8, table, ld_table, scale, out, s);
+    launch_lookup_of<float>(T, N, K, ids, id_bytes == 8, table, ld_table, scale, out, s);
   else if (type == HPSPMM_TYPE_F16)
-    launch_lookup_of<__half>(ctx, T, N, K, ids, id_bytes == 8, table, ld_table, scale, out, s);
+    launch_lookup_of<__half>(T, N, K, ids, id_bytes == 8, table, ld_table, scale, out, s);
   else
-    launch_lookup_of<__nv_bfloat16>(ctx, T, N, K, ids, id_bytes == 8, table, ld_table, scale, out, s);
+    launch_lookup_of<__nv_bfloat16>(T, N, K, ids, id_bytes == 8, table, ld_table, scale, out, s);
   ctx->launches++;
   HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
   return HPSPMM_OK;
@@ -542,7 +572,8 @@ int hpspmm_embedding_backward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, 
   const backward_plan p = plan_backward(T, N, K);
   HPSPMM_REQUIRE(ctx, T == 0 || workspace_bytes >= p.bytes, "workspace too small");
   HPSPMM_REQUIRE(ctx, T == 0 || ((uintptr_t)workspace & 255) == 0, "workspace not aligned to 256 bytes");
-  if (p.parts * ((K + 31) / 32) > (int64_t)2147483647 * 8) return hpspmm_unsupported(ctx, "more than 2^31 - 1 blocks");
+  if (p.parts * ((K + 31) / 32) > (int64_t)2147483647 * 8 || K > (int64_t)65535 * kJoinColumns)
+    return hpspmm_unsupported(ctx, "more than 2^31 - 1 blocks, or 8,388,480 columns");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   if (T == 0) {
