@@ -131,8 +131,9 @@ PROTOTYPES = {
     "hpspmm_embedding_backward": (c_int, [_P, _I64, _I64, _I64, c_int32, _P, c_int32, _P, _I64, c_float, _P, _P,
                                           c_size_t, _P]),
     "hpspmm_grouped_product": (c_int, [_P, _I64, _I64, _I64, _I64, c_int32, _P, _I64, _P, c_int32, _P, _P, _P]),
+    "hpspmm_grouped_weight_grad_workspace": (_I64, [_I64, _I64, _I64, _I64, c_int32, c_int32]),
     "hpspmm_grouped_weight_grad": (c_int, [_P, _I64, _I64, _I64, _I64, c_int32, _P, _I64, _P, _I64, _P, _P, c_int32,
-                                           _P]),
+                                           _P, c_size_t, _P]),
     "hpspmm_topk_distill_forward": (c_int, [_P, _I64, _I64, _I64, c_int32, _P, _I64, _P, c_int32, _P, c_float, _P, _P,
                                             _P]),
     "hpspmm_topk_distill_backward": (c_int, [_P, _I64, _I64, _I64, c_int32, _P, _I64, _P, c_int32, _P, c_float, _P, _P,
@@ -479,10 +480,11 @@ class Context:
                                                     int(w_out_first), _ptr(offsets), _ptr(Y), stream),
                     "hpspmm_grouped_product")
 
-    def grouped_weight_grad(self, R, G, K, N, dtype, X, ldx, dY, ldy, offsets, dW, w_out_first, stream=None):
+    def grouped_weight_grad(self, R, G, K, N, dtype, X, ldx, dY, ldy, offsets, dW, w_out_first, workspace=None,
+                            workspace_bytes=0, stream=None):
         self._check(self.lib.hpspmm_grouped_weight_grad(self.handle, R, G, K, N, dtype, _ptr(X), ldx, _ptr(dY), ldy,
-                                                        _ptr(offsets), _ptr(dW), int(w_out_first), stream),
-                    "hpspmm_grouped_weight_grad")
+                                                        _ptr(offsets), _ptr(dW), int(w_out_first), _ptr(workspace),
+                                                        workspace_bytes, stream), "hpspmm_grouped_weight_grad")
 
     def topk_distill_forward(self, T, V, k, dtype, logits, ld, ids, id_bytes, teacher, temperature, loss, stats=None,
                              stream=None):

@@ -27,7 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kLanes = 128;                    // columns of the output to a tile
 constexpr int kDepth = 64;                     // of one stage: 128 bytes, the span of the swizzle
 constexpr int kABytes = kLanes * kDepth * 2;
-constexpr int kMaxGroups = 2048;               // of one launch: their tile counts lie in shared memory
+constexpr int kMaxGroups = kMostSplitGroups;   // of one launch: their tile counts lie in shared memory
 constexpr int kMaxTiles = 0x7fff0000;          // of one launch: adding a grid to it stays within 31 bits
 constexpr int kMostTiles = 1 << 29;            // where the sum of the groups' tiles stops: two of them are below 2^31
 
@@ -40,6 +40,8 @@ struct tensor_args {
   int depth;           // products: K
   int rows, cols;      // of the output: products: -, N; gradients: rows and columns of one matrix
   int zero_rows;       // products: whether this launch clears the rows of no group
+  piece_plan plan;     // gradients
+  float* slots;
   int* timeouts;
 };
 
@@ -142,36 +144,51 @@ struct tile {
   int col0;            // of the output
   int begin, end;      // depth: products: stages of this block; gradients: rows of the group
   int stages;
+  int slot;            // gradients: where a piece of a group goes, -1: to the matrix itself
 };
 
 template <int MODE, int BN, int CL>
 __device__ __forceinline__ int tile_count(const tensor_args& a, const int* ends) {
   const int across = (a.cols + kLanes - 1) / kLanes;
-  if (MODE == MODE_WEIGHT) return a.gn * ((a.rows + BN - 1) / BN) * across;
+  if (MODE == MODE_WEIGHT)
+    return (int)min((int64_t)(a.plan.slots ? ends[a.gn - 1] : a.gn) * ((a.rows + BN - 1) / BN) * across, (int64_t)kMaxTiles);
   return (int)min((int64_t)ends[a.gn - 1] * across, (int64_t)kMaxTiles);
 }
 
 template <int MODE, int BN, int CL>
-__device__ __forceinline__ tile tile_at(const tensor_args& a, const int* ends, int u, int rank) {
+__device__ __forceinline__ tile tile_at(const tensor_args& a, const int* ends, const int* slot_ends, int u, int rank) {
   tile t;
   const int across = (a.cols + kLanes - 1) / kLanes;
-  const int q = u / across;
+  int q = u / across;
   t.col0 = (u - q * across) * kLanes;
+  t.slot = -1;
   if (MODE == MODE_WEIGHT) {
     const int down = (a.rows + BN - 1) / BN;
-    t.g = a.g0 + q / down;
     t.row0 = (q % down) * BN;
+    q /= down;
     t.rows = min(BN, a.rows - t.row0);
+  }
+  int lo = 0, hi = a.gn - 1;
+  if (MODE == MODE_WEIGHT && !a.plan.slots) {
+    lo = q;
+  } else {
+    while (lo < hi) {
+      const int m = (lo + hi) >> 1;
+      if (ends[m] > q) hi = m; else lo = m + 1;
+    }
+  }
+  t.g = a.g0 + lo;
+  if (MODE == MODE_WEIGHT) {
     part_bounds(a.offsets, a.G, a.R, t.g, t.begin, t.end);
+    if (a.plan.slots) {
+      const int piece = q - (lo ? ends[lo - 1] : 0);
+      if (pieces_of(max(t.end - t.begin, 0), a.plan.length) > 1) t.slot = (lo ? slot_ends[lo - 1] : 0) + piece;
+      t.begin += piece * a.plan.length;
+      t.end = min(t.end, t.begin + a.plan.length);
+    }
     t.stages = (max(t.end - t.begin, 0) + kDepth - 1) / kDepth;
     return t;
   }
-  int lo = 0, hi = a.gn - 1;
-  while (lo < hi) {
-    const int m = (lo + hi) >> 1;
-    if (ends[m] > q) hi = m; else lo = m + 1;
-  }
-  t.g = a.g0 + lo;
   const int first = lo ? ends[lo - 1] : 0, tiles = ends[lo] - first;
   int begin, end;
   part_bounds(a.offsets, a.G, a.R, t.g, begin, end);
@@ -211,6 +228,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   constexpr int kColumns = 2 * BN < 32 ? 32 : 2 * BN;                   // of tensor memory: two accumulators
   extern __shared__ char raw[];
   __shared__ int ends[kMaxGroups];
+  __shared__ int slot_ends[kWeight ? kMaxGroups : 1];
   __shared__ int part[kThreads / 32];
   __shared__ uint64_t bars[2 * STAGES + 6];
   __shared__ uint32_t tmem_base;
@@ -243,7 +261,8 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   }
   chain_grid();
 
-  if (!kWeight) {   // how many tiles the groups up to each one have
+  // How many tiles (pieces) the groups up to each one have, and how many slots
+  auto prefix = [&](int* to, bool slots) {
     constexpr int kPer = kMaxGroups / kThreads;
     int n[kPer], sum = 0;
 #pragma unroll
@@ -251,7 +270,12 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       const int g = threadIdx.x * kPer + i;
       int begin = 0, end = 0;
       if (g < a.gn) part_bounds(a.offsets, a.G, a.R, a.g0 + g, begin, end);
-      n[i] = (max(end - begin, 0) + BN - 1) / BN;
+      const int rows = max(end - begin, 0);
+      if (!kWeight)
+        n[i] = (rows + BN - 1) / BN;
+      else
+        n[i] = g < a.gn ? pieces_of(rows, a.plan.length) : 0;
+      if (slots && n[i] < 2) n[i] = 0;
       sum = min(sum + n[i], kMostTiles);
     }
     int before = sum;
@@ -267,9 +291,12 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       before = min(before + n[i], kMostTiles);
-      ends[threadIdx.x * kPer + i] = before;
+      to[threadIdx.x * kPer + i] = before;
     }
-  }
+    __syncthreads();
+  };
+  if (!kWeight || a.plan.slots) prefix(ends, false);
+  if (kWeight && a.plan.slots) prefix(slot_ends, true);
   __syncthreads();
   if (CL > 1) {   // the others' barriers are ready
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -286,7 +313,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       uint32_t phase = 0;
       bool ok = true;
       for (int u = first; u < units && ok; u += step) {
-        const tile t = tile_at<MODE, BN, CL>(a, ends, u, rank);
+        const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
         const int boxes = (t.rows + kBox - 1) / kBox;
         for (int k = 0; k < t.stages; ++k) {
           ok = mbar_wait(empty(s), phase ^ 1, &failed);
@@ -318,7 +345,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     int s = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     for (int u = first; u < units; u += step) {
-      const tile t = tile_at<MODE, BN, CL>(a, ends, u, rank);
+      const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
       if (!mbar_wait(acc_empty(acc), acc_phase ^ 1, &failed)) break;
       tensor_fence_after();
       const uint32_t d = tmem + acc * BN;
@@ -375,14 +402,28 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     int acc = 0;
     uint32_t acc_phase = 0, part_phase = 0;
     for (int u = first; u < units; u += step) {
-      const tile t = tile_at<MODE, BN, CL>(a, ends, u, rank);
+      const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
       if (!mbar_wait(acc_full(acc), acc_phase, &failed)) break;
       tensor_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(q * 32) << 16);
       const int col = t.col0 + q * 32 + lane;
       const bool inside = col < a.cols;
       T* to = out + (kWeight ? (int64_t)t.g * a.rows * a.cols : 0) + (int64_t)t.row0 * a.cols + col;
-      if (CL == 1) {
+      if (kWeight && t.slot >= 0) {   // a piece of a group, in 32 bits
+        float* piece = a.slots + (int64_t)t.slot * a.rows * a.cols + (int64_t)t.row0 * a.cols + col;
+        for (int c = 0; c < t.rows; c += 32) {
+          uint32_t v[32];
+          tensor_load(src + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (inside && c + j < t.rows && t.slot < a.plan.slots) *piece = __uint_as_float(v[j]);
+            piece += a.cols;
+          }
+        }
+        tensor_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty(acc));
+      } else if (CL == 1) {
         for (int c = 0; c < t.rows; c += 32) {
           uint32_t v[32];
           tensor_load(src + c, v);
@@ -530,7 +571,7 @@ bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // 0: launched, 1: this path does not take the call, otherwise a status
 int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx,
                                   const void* W, bool out_first, const int32_t* offsets, void* Y, cudaStream_t s) {
-  if (type == HPSPMM_TYPE_F32 || K % 8 || N % 8 || ldx % 8 || ldx < K || G == 0 || K == 0 || !aligned(X) || !aligned(W) || !aligned(Y))
+  if (type == HPSPMM_TYPE_F32 || K % 8 || N % 8 || ldx % 8 || ldx < K || !aligned(X) || !aligned(W) || !aligned(Y))
     return 1;
   const bool half = type == HPSPMM_TYPE_F16;
   const bool wide = R > 64 * G;
@@ -545,7 +586,8 @@ int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t
   if ((R / bn + G + 1) * across > kMaxTiles || R / bn + G + 1 > kMostTiles) return 1;
   for (int64_t g0 = 0; g0 < G; g0 += kMaxGroups) {
     const int64_t gn = std::min<int64_t>(kMaxGroups, G - g0);
-    const tensor_args a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
+    const tensor_args a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, {(int)R, 0}, nullptr,
+                           ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
     const int64_t units = (std::min(R, gn) + R / bn) * across;   // no more than that
     cudaError_t e;
     if (half)
@@ -561,17 +603,18 @@ int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t
 
 // dW[g] (I x J) = A_g^T * B_g with A R x I and B R x J
 int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t I, int64_t J, int32_t type, const void* A,
-                                      int64_t lda, const void* B, int64_t ldb, const int32_t* offsets, void* dW, cudaStream_t s) {
-  if (type == HPSPMM_TYPE_F32 || R == 0 || I % 8 || J % 8 || lda % 8 || ldb % 8 || lda < I || ldb < J || !aligned(A) || !aligned(B))
+                                      int64_t lda, const void* B, int64_t ldb, const int32_t* offsets, void* dW,
+                                      const piece_plan& p, float* slots, cudaStream_t s) {
+  if (type == HPSPMM_TYPE_F32 || I % 8 || J % 8 || lda % 8 || ldb % 8 || lda < I || ldb < J || !aligned(A) || !aligned(B))
     return 1;
   const bool half = type == HPSPMM_TYPE_F16;
   CUtensorMap ma, mb;   // the operand of the output's columns lies on the lanes
   const int64_t asize[2] = {J, R}, astride[1] = {ldb}, bsize[2] = {I, R}, bstride[1] = {lda};
   const int box[2] = {64, kDepth};
   if (!encode(&ma, half, B, 2, asize, astride, box) || !encode(&mb, half, A, 2, bsize, bstride, box)) return 1;
-  const int64_t units = G * ((I + 255) / 256) * ((J + kLanes - 1) / kLanes);
+  const int64_t units = (G + p.slots) * ((I + 255) / 256) * ((J + kLanes - 1) / kLanes);
   if (units > kMaxTiles) return 1;
-  const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
+  const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, p, slots, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
   const cudaError_t e = half ? launch_one<__half, MODE_WEIGHT, 256, 4, 1>(ctx, a, ma, mb, dW, units, s)
                              : launch_one<__nv_bfloat16, MODE_WEIGHT, 256, 4, 1>(ctx, a, ma, mb, dW, units, s);
   HPSPMM_CUDA_TRY(ctx, e);

@@ -149,10 +149,13 @@ Tensor grouped_weight_grad(const Tensor& X, const Tensor& dY, const Tensor& offs
   const Tensor offsets = offsets_of(offsets_, X.device(), groups), x = rows_of(X), dy = rows_of(dY);
   const int64_t K = x.size(1), N = dy.size(1);
   Tensor dW = transposed ? at::empty({groups, N, K}, x.options()) : at::empty({groups, K, N}, x.options());
+  const int64_t bytes = hpspmm_grouped_weight_grad_workspace(x.size(0), groups, K, N, type, transposed);
+  TORCH_CHECK(bytes >= 0, "hpspmm: more than 2^31 - 2 rows or columns, or 2^20 groups");
+  const Tensor workspace = at::empty({bytes}, x.options().dtype(at::kByte));
   call(x.device(), "hpspmm_grouped_weight_grad", [&](hpspmm_ctx* ctx, hpspmm_stream stream) {
     return hpspmm_grouped_weight_grad(ctx, x.size(0), groups, K, N, type, x.const_data_ptr(), stride_of(x),
                                       dy.const_data_ptr(), stride_of(dy), offsets.const_data_ptr<int>(),
-                                      dW.mutable_data_ptr(), transposed, stream);
+                                      dW.mutable_data_ptr(), transposed, workspace.mutable_data_ptr(), (size_t)bytes, stream);
   });
   return transposed ? dW.transpose(1, 2) : dW;
 }

@@ -355,11 +355,17 @@ HPSPMM_API int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int
                                       int32_t type, const void* X, int64_t ldx, const void* W,
                                       int32_t w_out_first, const int32_t* offsets, void* Y,
                                       hpspmm_stream stream);
-/* dW[g] = X_g^T * dY_g over the rows of group g, stored as w_out_first says; zeros for a group without rows. */
+/* dW[g] = X_g^T * dY_g over the rows of group g, stored as w_out_first says; zeros for a group without rows.  Groups of
+ * many rows are cut into pieces where the matrices alone would not fill the GPU; their sums wait in workspace: device
+ * memory of hpspmm_grouped_weight_grad_workspace bytes (0 where none is needed, -1: a size or type is not accepted),
+ * aligned to 256 bytes, that no other call uses until this one is done; it needs no initial value. */
+HPSPMM_API int64_t hpspmm_grouped_weight_grad_workspace(int64_t R, int64_t G, int64_t K, int64_t N,
+                                                        int32_t type, int32_t w_out_first);
 HPSPMM_API int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N,
                                           int32_t type, const void* X, int64_t ldx, const void* dY,
                                           int64_t ldy, const int32_t* offsets, void* dW,
-                                          int32_t w_out_first, hpspmm_stream stream);
+                                          int32_t w_out_first, void* workspace, size_t workspace_bytes,
+                                          hpspmm_stream stream);
 
 /* For every row z of T x V logits and the k entries (ids[j], teacher_logits[j]) its teacher kept:
  *   p    = softmax over the entries of teacher_logits / temperature

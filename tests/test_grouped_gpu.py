@@ -264,7 +264,39 @@ def test_refusals(ops, pkg, gpu_ctx):
         with pytest.raises(pkg.HpspmmError):
             gpu_ctx.grouped_product(*(good[:at] + [v] + good[at + 1:]))
     good = [6, 2, 8, 4, pkg.TYPE_F32, X.data_ptr(), 8, Y.data_ptr(), 4, off.data_ptr(), W.data_ptr(), 0]
-    gpu_ctx.grouped_weight_grad(*good)
+    gpu_ctx.grouped_weight_grad(*good)                # so few rows are not cut into pieces
     for at, v in ((0, -1), (4, -1), (5, None), (6, -1), (7, None), (8, -1), (9, None), (10, None), (1, 1 << 40)):
         with pytest.raises(pkg.HpspmmError):
             gpu_ctx.grouped_weight_grad(*(good[:at] + [v] + good[at + 1:]))
+    size = pkg.load_library().hpspmm_grouped_weight_grad_workspace
+    for dtype in (pkg.TYPE_F32, pkg.TYPE_BF16):
+        assert size(0, 3, 8, 8, dtype, 0) == 0 and size(100, 3, 8, 8, dtype, 1) == 0
+        assert size(-1, 3, 8, 8, dtype, 0) == -1 and size(5, 3, 8, 8, 9, 0) == -1
+        need = size(20_000, 3, 64, 32, dtype, 0)
+        assert 0 < need <= 20_000 * 96 * 4
+    X, Y, W = torch.zeros((20_000, 64), device="cuda"), torch.zeros((20_000, 32), device="cuda"), torch.zeros((3, 64, 32), device="cuda")
+    off = _offsets([10_000, 0, 10_000])
+    need = size(20_000, 3, 64, 32, pkg.TYPE_F32, 0)
+    space = torch.zeros(need + 256, dtype=torch.uint8, device="cuda")
+    good = [20_000, 3, 64, 32, pkg.TYPE_F32, X.data_ptr(), 64, Y.data_ptr(), 32, off.data_ptr(), W.data_ptr(), 0, space.data_ptr(), need]
+    gpu_ctx.grouped_weight_grad(*good)
+    for at, v in ((12, None), (13, need - 1), (12, space.data_ptr() + 4)):
+        with pytest.raises(pkg.HpspmmError):
+            gpu_ctx.grouped_weight_grad(*(good[:at] + [v] + good[at + 1:]))
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("sizes,K,N", [([5000], 64, 40), ([0, 9000, 3, 2049, 0, 1024], 136, 64), ([4097, 7000], 33, 50), ([30_000, 1], 256, 264)])
+def test_groups_cut_into_pieces(ops, type, sizes, K, N):
+    """Few matrices and many rows: the gradient of a matrix is a sum over pieces of its group."""
+    gen = torch.Generator("cuda").manual_seed(K)
+    for transposed in (False, True):
+        X, dY = (torch.randn((sum(sizes) + 3, c), device="cuda", generator=gen).to(ref.TYPES[type]) for c in (K, N))
+        W = _weights(len(sizes), K, N, X.dtype, gen, transposed)
+        _, _, first = _check(ops, X, W, _offsets(sizes), dY)
+        _, _, again = _check(ops, X, W, _offsets(sizes), dY)
+        assert torch.equal(first, again)
+    # offsets that do not ascend want more pieces than there is room for
+    n = sum(sizes)
+    off = torch.tensor([0, n] * 3 + [0], dtype=torch.int32, device="cuda")
+    assert torch.ops.hpspmm.grouped_weight_grad(X, dY, off, False).shape == (6, K, N)
