@@ -41,7 +41,7 @@ static inline int64_t piece_slots(int64_t R, int64_t length) { return length >= 
 int hpspmm_join_pieces(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t elements, int32_t type, const int32_t* offsets,
                        const hpspmm::piece_plan& p, const float* slots, void* dW, cudaStream_t s);
 
-// The tensor-core kernels.  0: launched, 1: the call is not for them (types, alignment), otherwise a status.
+// The tensor-core kernels, for 16-bit types.
 int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx,
                                   const void* W, bool out_first, const int32_t* offsets, void* Y, cudaStream_t s);
 int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t I, int64_t J, int32_t type, const void* A,

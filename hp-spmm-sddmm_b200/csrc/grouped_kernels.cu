@@ -100,16 +100,16 @@ __device__ __forceinline__ uint64_t both(float v) {
 
 // ROWS x 16 elements of an operand; element (i, k) lies at p[i * stride + k] (ALONG: next to each other along the depth) or
 // p[k * stride + i].  VEC: four neighbours are one aligned load, or none of them is there.
-template <typename T, int ROWS, bool ALONG, bool VEC>
+template <int ROWS, bool ALONG, bool VEC>
 struct tile_loader {
   static constexpr int kEach = ROWS * kTileDepth / kThreads / 4;   // quads to a thread
   float v[kEach][4];
-  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int depth, int k0) {
+  __device__ __forceinline__ void load(const float* p, int64_t stride, int rows, int depth, int k0) {
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
       const int q = threadIdx.x + u * kThreads;
       const int i = ALONG ? q >> 2 : q % (ROWS / 4) * 4, k = k0 + (ALONG ? (q & 3) * 4 : q / (ROWS / 4));
-      const T* at = p + (ALONG ? i * stride + k : k * stride + i);
+      const float* at = p + (ALONG ? i * stride + k : k * stride + i);
       const bool line = ALONG ? i < rows : k < depth;
       const int left = !line ? 0 : (ALONG ? depth - k : rows - i);
       if (VEC) {
@@ -118,7 +118,7 @@ struct tile_loader {
         v[u][0] = x.x, v[u][1] = x.y, v[u][2] = x.z, v[u][3] = x.w;
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[u][e] = e < left ? to_float(at[e]) : 0.f;
+        for (int e = 0; e < 4; ++e) v[u][e] = e < left ? __ldg(at + e) : 0.f;
       }
     }
   }
@@ -136,9 +136,9 @@ struct tile_loader {
   }
 };
 
-// C[i][j] = sum over k < depth of A(i, k) * B(k, j) for i < rows, j < cols; OUT is what C is stored as.
-template <typename T, typename OUT, int BN, bool A_ALONG, bool B_ALONG, bool VEC>
-__device__ __forceinline__ void tile_product(const T* A, int64_t sa, const T* B, int64_t sb, int rows, int cols, int depth, OUT* C,
+// C[i][j] = sum over k < depth of A(i, k) * B(k, j) for i < rows, j < cols.
+template <int BN, bool A_ALONG, bool B_ALONG, bool VEC>
+__device__ __forceinline__ void tile_product(const float* A, int64_t sa, const float* B, int64_t sb, int rows, int cols, int depth, float* C,
                                              int64_t sc, float (*As)[kTileDepth][kTileRows + 4], float (*Bs)[kTileDepth][BN + 4]) {
   constexpr int kHalves = BN / 64;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -147,8 +147,8 @@ __device__ __forceinline__ void tile_product(const T* A, int64_t sa, const T* B,
   for (int x = 0; x < 8; ++x)
 #pragma unroll
     for (int y = 0; y < kHalves * 2; ++y) acc[x][y] = 0;
-  tile_loader<T, kTileRows, A_ALONG, VEC> la;
-  tile_loader<T, BN, B_ALONG, VEC> lb;
+  tile_loader<kTileRows, A_ALONG, VEC> la;
+  tile_loader<BN, B_ALONG, VEC> lb;
   la.load(A, sa, rows, depth, 0), lb.load(B, sb, cols, depth, 0);
   la.store(As[0]), lb.store(Bs[0]);
   __syncthreads();
@@ -185,7 +185,7 @@ __device__ __forceinline__ void tile_product(const T* A, int64_t sa, const T* B,
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       const int j = tx * 4 + 64 * h;
-      OUT* to = C + (int64_t)i * sc + j;
+      float* to = C + (int64_t)i * sc + j;
       float v[4];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -197,16 +197,16 @@ __device__ __forceinline__ void tile_product(const T* A, int64_t sa, const T* B,
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (j + e < cols) to[e] = from_float<OUT>(v[e]);
+          if (j + e < cols) to[e] = v[e];
       }
     }
   }
 }
 
-template <typename T, int BN, bool OUT_FIRST, bool VEC>
+template <int BN, bool OUT_FIRST, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2)
-grouped_product_kernel(int R, int G, int K, int N, const T* __restrict__ X, int64_t ldx, const T* __restrict__ W, const int* offsets,
-                       T* __restrict__ Y, int col_tiles) {
+grouped_product_kernel(int R, int G, int K, int N, const float* __restrict__ X, int64_t ldx, const float* __restrict__ W, const int* offsets,
+                       float* __restrict__ Y, int col_tiles) {
   __shared__ float As[2][kTileDepth][kTileRows + 4], Bs[2][kTileDepth][BN + 4];
   __shared__ row_tile shared_tile;
   const int t = blockIdx.x / col_tiles, j0 = (blockIdx.x - t * col_tiles) * BN;
@@ -218,16 +218,16 @@ grouped_product_kernel(int R, int G, int K, int N, const T* __restrict__ X, int6
   const row_tile w = shared_tile;
   if (w.rows == 0) return;
   const bool none = w.g >= G;
-  const T* wg = none ? W : W + (int64_t)w.g * K * N;
-  tile_product<T, T, BN, true, OUT_FIRST, VEC>(X + (int64_t)w.r0 * ldx, ldx, OUT_FIRST ? wg + (int64_t)j0 * K : wg + j0, OUT_FIRST ? K : N,
+  const float* wg = none ? W : W + (int64_t)w.g * K * N;
+  tile_product<BN, true, OUT_FIRST, VEC>(X + (int64_t)w.r0 * ldx, ldx, OUT_FIRST ? wg + (int64_t)j0 * K : wg + j0, OUT_FIRST ? K : N,
                                                w.rows, min(BN, N - j0), none ? 0 : K, Y + (int64_t)w.r0 * N + j0, N, As, Bs);
 }
 
 // dW[g][i][j] = sum over the rows of the group of A[r][i] * B[r][j]
-template <typename T, int BN, bool VEC>
+template <int BN, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2)
-grouped_weight_grad_kernel(int R, int G, int I, int J, const T* __restrict__ A, int64_t lda, const T* __restrict__ B, int64_t ldb,
-                           const int* offsets, T* __restrict__ dW, const piece_plan plan, float* slots, int i_tiles, int j_tiles) {
+grouped_weight_grad_kernel(int R, int G, int I, int J, const float* __restrict__ A, int64_t lda, const float* __restrict__ B, int64_t ldb,
+                           const int* offsets, float* __restrict__ dW, const piece_plan plan, float* slots, int i_tiles, int j_tiles) {
   __shared__ float As[2][kTileDepth][kTileRows + 4], Bs[2][kTileDepth][BN + 4];
   __shared__ row_tile shared_tile;
   int t = blockIdx.x;
@@ -242,13 +242,10 @@ grouped_weight_grad_kernel(int R, int G, int I, int J, const T* __restrict__ A, 
   __syncthreads();
   const row_tile w = shared_tile;
   if (w.pieces == 0 || (w.pieces > 1 && w.slot >= plan.slots)) return;
-  const T *a = A + (int64_t)w.r0 * lda + i0, *b = B + (int64_t)w.r0 * ldb + j0;
+  const float *a = A + (int64_t)w.r0 * lda + i0, *b = B + (int64_t)w.r0 * ldb + j0;
   const int rows = min(kTileRows, I - i0), cols = min(BN, J - j0);
-  const int64_t at = (int64_t)i0 * J + j0;
-  if (w.pieces == 1)
-    tile_product<T, T, BN, false, false, VEC>(a, lda, b, ldb, rows, cols, w.rows, dW + (int64_t)w.g * I * J + at, J, As, Bs);
-  else
-    tile_product<T, float, BN, false, false, VEC>(a, lda, b, ldb, rows, cols, w.rows, slots + (int64_t)w.slot * I * J + at, J, As, Bs);
+  float* to = w.pieces == 1 ? dW + (int64_t)w.g * I * J : slots + (int64_t)w.slot * I * J;
+  tile_product<BN, false, false, VEC>(a, lda, b, ldb, rows, cols, w.rows, to + (int64_t)i0 * J + j0, J, As, Bs);
 }
 
 // Groups of more than one piece: the pieces in order.
@@ -283,21 +280,21 @@ join_pieces_kernel(int R, int G, int64_t elements, const int* offsets, const pie
   }
 }
 
-template <typename T, int BN, bool OUT_FIRST, bool VEC>
+template <int BN, bool OUT_FIRST, bool VEC>
 void launch_product(int64_t R, int64_t G, int64_t K, int64_t N, const void* X, int64_t ldx, const void* W, const int32_t* offsets,
                     void* Y, cudaStream_t s) {
   const int64_t col_tiles = (N + BN - 1) / BN, blocks = ((R + kTileRows - 1) / kTileRows + G + 2) * col_tiles;
-  grouped_product_kernel<T, BN, OUT_FIRST, VEC><<<(unsigned)blocks, kThreads, 0, s>>>((int)R, (int)G, (int)K, (int)N, (const T*)X, ldx,
-                                                                                     (const T*)W, offsets, (T*)Y, (int)col_tiles);
+  grouped_product_kernel<BN, OUT_FIRST, VEC><<<(unsigned)blocks, kThreads, 0, s>>>((int)R, (int)G, (int)K, (int)N, (const float*)X, ldx,
+                                                                                  (const float*)W, offsets, (float*)Y, (int)col_tiles);
 }
 
-template <typename T, int BN, bool VEC>
+template <int BN, bool VEC>
 void launch_weight_grad(int64_t R, int64_t G, int64_t I, int64_t J, const void* A, int64_t lda, const void* B, int64_t ldb,
                         const int32_t* offsets, void* dW, const piece_plan& p, float* slots, cudaStream_t s) {
   const int64_t i_tiles = (I + kTileRows - 1) / kTileRows, j_tiles = (J + BN - 1) / BN;
   const int64_t blocks = (G + piece_slots(R, p.length)) * i_tiles * j_tiles;
-  grouped_weight_grad_kernel<T, BN, VEC><<<(unsigned)blocks, kThreads, 0, s>>>((int)R, (int)G, (int)I, (int)J, (const T*)A, lda,
-                                                                              (const T*)B, ldb, offsets, (T*)dW, p, slots, (int)i_tiles,
+  grouped_weight_grad_kernel<BN, VEC><<<(unsigned)blocks, kThreads, 0, s>>>((int)R, (int)G, (int)I, (int)J, (const float*)A, lda,
+                                                                           (const float*)B, ldb, offsets, (float*)dW, p, slots, (int)i_tiles,
                                                                               (int)j_tiles);
 }
 
@@ -343,13 +340,13 @@ int hpspmm_join_pieces(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t elements, 
   return HPSPMM_OK;
 }
 
-template <typename T, int BN, bool VEC>
+template <int BN, bool VEC>
 void launch_product(bool out_first, int64_t R, int64_t G, int64_t K, int64_t N, const void* X, int64_t ldx, const void* W,
                     const int32_t* offsets, void* Y, cudaStream_t s) {
   if (out_first)
-    launch_product<T, BN, true, VEC>(R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<BN, true, VEC>(R, G, K, N, X, ldx, W, offsets, Y, s);
   else
-    launch_product<T, BN, false, VEC>(R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<BN, false, VEC>(R, G, K, N, X, ldx, W, offsets, Y, s);
 }
 
 extern "C" {
@@ -370,24 +367,20 @@ int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int
     HPSPMM_CUDA_TRY(ctx, cudaMemsetAsync(Y, 0, (size_t)(R * N) * dense_type_size(type), s));
     return HPSPMM_OK;
   }
-  const int done = hpspmm_grouped_product_tensor(ctx, R, G, K, N, type, X, ldx, W, w_out_first != 0, offsets, Y, s);
-  if (done != 1) return done;
+  if (type != HPSPMM_TYPE_F32)
+    return hpspmm_grouped_product_tensor(ctx, R, G, K, N, type, X, ldx, W, w_out_first != 0, offsets, Y, s);
   if (((R + kTileRows - 1) / kTileRows + G + 2) * ((N + 63) / 64) > 2147483647ll)
     return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 128 x 64");
-  const bool vec = type == HPSPMM_TYPE_F32 && K % 4 == 0 && N % 4 == 0 && ldx % 4 == 0 && aligned16(X) && aligned16(W) && aligned16(Y);
+  const bool vec = K % 4 == 0 && N % 4 == 0 && ldx % 4 == 0 && aligned16(X) && aligned16(W) && aligned16(Y);
   const bool narrow = tile_columns(N) == 64, of = w_out_first != 0;
-  if (type == HPSPMM_TYPE_F16)
-    launch_product<__half, 128, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
-  else if (type == HPSPMM_TYPE_BF16)
-    launch_product<__nv_bfloat16, 128, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
-  else if (vec && narrow)
-    launch_product<float, 64, true>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+  if (vec && narrow)
+    launch_product<64, true>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (vec)
-    launch_product<float, 128, true>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<128, true>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (narrow)
-    launch_product<float, 64, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<64, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
   else
-    launch_product<float, 128, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<128, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
   ctx->launches++;
   HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
   return HPSPMM_OK;
@@ -425,29 +418,25 @@ int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K,
     HPSPMM_REQUIRE(ctx, workspace != nullptr && (int64_t)workspace_bytes >= (int64_t)p.slots * K * N * 4, "workspace too small");
     HPSPMM_REQUIRE(ctx, ((uintptr_t)workspace & 255) == 0, "workspace not aligned to 256 bytes");
   }
-  const int done = hpspmm_grouped_weight_grad_tensor(ctx, R, G, I, J, type, A, lda, B, ldb, offsets, dW, p, slots, s);
-  if (done == 1) {
+  if (type != HPSPMM_TYPE_F32) {
+    const int done = hpspmm_grouped_weight_grad_tensor(ctx, R, G, I, J, type, A, lda, B, ldb, offsets, dW, p, slots, s);
+    if (done != HPSPMM_OK) return done;
+  } else {
     if ((G + p.slots) * ((I + kTileRows - 1) / kTileRows) * ((J + 63) / 64) > 2147483647ll)
       return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 128 x 64");
-    const bool vec = type == HPSPMM_TYPE_F32 && I % 4 == 0 && J % 4 == 0 && lda % 4 == 0 && ldb % 4 == 0 && aligned16(A) && aligned16(B) &&
+    const bool vec = I % 4 == 0 && J % 4 == 0 && lda % 4 == 0 && ldb % 4 == 0 && aligned16(A) && aligned16(B) &&
                      aligned16(dW);
     const bool narrow = tile_columns(J) == 64;
-    if (type == HPSPMM_TYPE_F16)
-      launch_weight_grad<__half, 128, false>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
-    else if (type == HPSPMM_TYPE_BF16)
-      launch_weight_grad<__nv_bfloat16, 128, false>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
-    else if (vec && narrow)
-      launch_weight_grad<float, 64, true>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
+    if (vec && narrow)
+      launch_weight_grad<64, true>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
     else if (vec)
-      launch_weight_grad<float, 128, true>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
+      launch_weight_grad<128, true>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
     else if (narrow)
-      launch_weight_grad<float, 64, false>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
+      launch_weight_grad<64, false>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
     else
-      launch_weight_grad<float, 128, false>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
+      launch_weight_grad<128, false>(R, G, I, J, A, lda, B, ldb, offsets, dW, p, slots, s);
     ctx->launches++;
     HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
-  } else if (done != HPSPMM_OK) {
-    return done;
   }
   return p.slots > 0 ? hpspmm_join_pieces(ctx, R, G, K * N, type, offsets, p, slots, dW, s) : HPSPMM_OK;
 }

@@ -43,6 +43,9 @@ struct tensor_args {
   piece_plan plan;     // gradients
   float* slots;
   int* timeouts;
+  // the operands on the lanes and on the N side, for calls whose tiles TMA cannot fetch: rows ld elements apart
+  const void *a, *b;
+  int64_t lda, ldb;
 };
 
 // ---- instructions ------------------------------------------------------------------------------------------------
@@ -215,11 +218,59 @@ struct type_code<__nv_bfloat16> { static constexpr uint32_t value = 1; };
 template <int BN>
 __host__ __device__ constexpr int box_rows() { return BN >= 128 ? 64 : 16; }
 
+// ---- tiles without TMA ---------------------------------------------------------------------------------------------
+//
+// Operands whose rows do not begin on 16-byte boundaries: eight warps bring a tile in, two such teams in turn, 128 bytes of
+// neighbouring elements to a warp, two to a lane, and write it swizzled as TMA does.  Loads go without a branch, from an element that is
+// there where the wanted one is not: conditional loads of one batch waited for one another, 0.7 us each.  (Aligned words,
+// shifted by half a word where a row begins in the middle of one, took a third of the loads and ten times the
+// instructions: 78 us where this takes 22.9, for 5,003 rows of 13 groups, 333 x 131.)
+
+constexpr int kLoaders = 8;     // warps of a team
+constexpr int kTeams = 2;
+constexpr int kLinesInFlight = 16;
+
+// Lines `warp`, `warp` + kLoaders, ... of an operand's tile.  Line i holds 64 elements of row `row + i % PER` (there is none
+// from `rows` on) from column `col + 64 * (i / PER)` (there is none from `cols` on): zeros stand for what is not there.
+template <int PER>
+__device__ __forceinline__ void load_lines(const uint16_t* p, int64_t ld, int warp, int lines, int64_t row, int64_t rows, int col, int cols,
+                                           uint32_t tile) {
+  const int lane = threadIdx.x & 31, present = (int)min(rows - row, (int64_t)PER);
+  for (int first = 0; first < lines; first += PER) {
+    const int c = col + 64 * (first / PER), valid = min(max(cols - c, 0), 64), n = min(PER, lines - first);
+    // the lane's elements, and which of them count
+    const int e0 = min(2 * lane, valid - 1), e1 = min(2 * lane + 1, valid - 1);
+    const uint32_t keep = (2 * lane < valid ? 0xffffu : 0u) | (2 * lane + 1 < valid ? 0xffff0000u : 0u);
+    const uint16_t* from = p + row * ld + c;
+    for (int i0 = warp; i0 < n; i0 += kLoaders * kLinesInFlight) {
+      uint32_t low[kLinesInFlight], high[kLinesInFlight];
+#pragma unroll
+      for (int j = 0; j < kLinesInFlight; ++j) low[j] = high[j] = 0;
+      if (valid > 0) {
+#pragma unroll
+        for (int j = 0; j < kLinesInFlight; ++j) {
+          const uint16_t* at = from + min(i0 + j * kLoaders, present - 1) * ld;
+          low[j] = __ldg(at + e0), high[j] = __ldg(at + e1);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kLinesInFlight; ++j) {
+        const int i = i0 + j * kLoaders;
+        if (i < n) {
+          const uint32_t v = i < present ? (low[j] | high[j] << 16) & keep : 0;
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(tile + (first + i) * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4), "r"(v)
+                       : "memory");
+        }
+      }
+    }
+  }
+}
+
 template <int BN, int STAGES, int CL>
 constexpr int smem_bytes() { return 1024 + STAGES * (kABytes + BN * 128) + (CL > 1 ? BN * kLanes * 4 : 0); }
 
-template <typename T, int MODE, int BN, int STAGES, int CL>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int MODE, int BN, int STAGES, int CL, bool TMA>
+__global__ void __launch_bounds__(TMA ? kThreads : kThreads + kTeams * kLoaders * 32, 1)
 grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                       T* __restrict__ out) {
   constexpr bool kWeight = MODE == MODE_WEIGHT;
@@ -247,12 +298,14 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
 
   if (threadIdx.x == 0) {
     failed = 0;
-    for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+    for (int s = 0; s < STAGES; ++s) mbar_init(full(s), TMA ? 1 : kLoaders), mbar_init(empty(s), 1);
     for (int b = 0; b < 2; ++b) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 4);
     mbar_init(parts_full, 4 * CL), mbar_init(parts_empty, 4 * CL);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    if (TMA) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    }
   }
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&tmem_base)), "n"(kColumns) : "memory");
@@ -264,10 +317,11 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   // How many tiles (pieces) the groups up to each one have, and how many slots
   auto prefix = [&](int* to, bool slots) {
     constexpr int kPer = kMaxGroups / kThreads;
+    const bool counts = TMA || threadIdx.x < kThreads;
     int n[kPer], sum = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int g = threadIdx.x * kPer + i;
+      const int g = counts ? threadIdx.x * kPer + i : a.gn;
       int begin = 0, end = 0;
       if (g < a.gn) part_bounds(a.offsets, a.G, a.R, a.g0 + g, begin, end);
       const int rows = max(end - begin, 0);
@@ -284,14 +338,16 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       const int o = __shfl_up_sync(0xffffffffu, before, d);
       if (lane >= d) before = min(before + o, kMostTiles);
     }
-    if (lane == 31) part[warp] = before;
+    if (counts && lane == 31) part[warp] = before;
     __syncthreads();
     before = max(before - sum, 0);
-    for (int w = 0; w < warp; ++w) before = min(before + part[w], kMostTiles);
+    if (counts) {
+      for (int w = 0; w < warp; ++w) before = min(before + part[w], kMostTiles);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      before = min(before + n[i], kMostTiles);
-      to[threadIdx.x * kPer + i] = before;
+      for (int i = 0; i < kPer; ++i) {
+        before = min(before + n[i], kMostTiles);
+        to[threadIdx.x * kPer + i] = before;
+      }
     }
     __syncthreads();
   };
@@ -308,7 +364,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   const int first = blockIdx.x / CL, step = gridDim.x / CL;
 
   if (warp == 0) {
-    if (lane == 0) {   // copies
+    if (TMA && lane == 0) {   // copies
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -362,7 +418,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         int left;   // of the depth in this stage
         if (kWeight) {
           left = t.end - t.begin - k * kDepth;
-          if (left < kDepth && (left & 15)) {   // the next group's rows, up to the end of the instruction's depth, become zeros
+          if (TMA && left < kDepth && (left & 15)) {   // the next group's rows, up to the end of the instruction's depth, become zeros
             const int wide = 2 + (t.rows + 63) / 64, rows = 16 - (left & 15);
             for (int i = lane; i < wide * rows * 8; i += 32) {
               const int b = i / (rows * 8), r = left + (i >> 3) % rows;
@@ -396,6 +452,41 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       __syncwarp();
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
+    }
+  } else if (!TMA && warp >= kThreads / 32) {   // copies, line by line
+    const int w = (warp - kThreads / 32) % kLoaders, team = (warp - kThreads / 32) / kLoaders;
+    const uint16_t *pa = static_cast<const uint16_t*>(a.a), *pb = static_cast<const uint16_t*>(a.b);
+    int s = 0, turn = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int u = first; u < units && ok; u += step) {
+      const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
+      for (int k = 0; k < t.stages; ++k) {
+        const int at = s;
+        const uint32_t parity = phase ^ 1;
+        if (++s == STAGES) s = 0, phase ^= 1;
+        turn = turn + 1 == kTeams ? 0 : turn + 1;
+        if (turn != team) continue;
+        ok = mbar_wait(empty(at), parity, &failed);
+        if (!ok) break;
+        const uint32_t dst = base + at * kStage;
+        if (kWeight) {
+          const int64_t r = (int64_t)t.begin + k * kDepth;
+          load_lines<kDepth>(pa, a.lda, w, kLanes, r, t.end, t.col0, a.cols, dst);
+          load_lines<kDepth>(pb, a.ldb, w, (t.rows + 63) / 64 * kDepth, r, t.end, t.row0, a.rows, dst + kABytes);
+        } else {
+          const int d = (t.begin + k) * kDepth;
+          const uint16_t* wg = pa + (int64_t)t.g * a.depth * a.cols;
+          if (MODE == MODE_OUT_FIRST)
+            load_lines<kLanes>(wg, a.lda, w, kLanes, t.col0, a.cols, d, a.depth, dst);
+          else
+            load_lines<kDepth>(wg, a.lda, w, kLanes, d, a.depth, t.col0, a.cols, dst);
+          load_lines<BN>(pb, a.ldb, w, t.rows, t.row0, a.R, d, a.depth, dst + kABytes);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(at));
+      }
     }
   } else if (warp >= 4) {   // results
     const int q = warp - 4;
@@ -481,13 +572,14 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       if (acc == 0) acc_phase ^= 1;
     }
   } else if (!kWeight && a.zero_rows) {   // rows of no group, by the two warps that are left
-    const int64_t width = a.cols / 8;     // 16-byte words to a row
-    uint4* words = reinterpret_cast<uint4*>(out);
+    typedef typename raw_bytes<TMA ? 16 : 2>::type word;
+    const int64_t width = TMA ? a.cols / 8 : a.cols;     // words to a row
+    word* words = reinterpret_cast<word*>(out);
     const int64_t at = (int64_t)blockIdx.x * 64 + (threadIdx.x - 64), all = (int64_t)gridDim.x * 64;
     for (int i = a.G; i < a.G + 2; ++i) {
       int begin, end;
       part_bounds(a.offsets, a.G, a.R, i, begin, end);
-      for (int64_t w = begin * width + at; w < end * width; w += all) words[w] = make_uint4(0, 0, 0, 0);
+      for (int64_t w = begin * width + at; w < end * width; w += all) words[w] = word{};
     }
   }
   tensor_fence_before();
@@ -529,10 +621,10 @@ bool encode(CUtensorMap* map, bool half, const void* p, int dims, const int64_t*
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int MODE, int BN, int STAGES, int CL>
+template <typename T, int MODE, int BN, int STAGES, int CL, bool TMA>
 cudaError_t launch_one(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* out, int64_t units,
                        cudaStream_t s) {
-  auto* kernel = grouped_tensor_kernel<T, MODE, BN, STAGES, CL>;
+  auto* kernel = grouped_tensor_kernel<T, MODE, BN, STAGES, CL, TMA>;
   constexpr int smem = smem_bytes<BN, STAGES, CL>();
   // per call: the attribute belongs to the current device's context, and a process may drive several GPUs
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -544,59 +636,76 @@ cudaError_t launch_one(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap&
   attr[1].val.clusterDim.x = CL, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3((unsigned)(std::min<int64_t>(units, ctx->sm_count / CL) * CL));
-  c.blockDim = dim3(kThreads);
+  c.blockDim = dim3(TMA ? kThreads : kThreads + kTeams * kLoaders * 32);
   c.dynamicSmemBytes = smem, c.stream = s, c.attrs = attr, c.numAttrs = CL > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&c, kernel, a, ma, mb, (T*)out);
   ctx->launches++;
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T, int MODE>
-cudaError_t launch_product(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* out, bool wide,
-                           int64_t units, cudaStream_t s) {
-  if (wide) return launch_one<T, MODE, 256, 4, 1>(ctx, a, ma, mb, out, units, s);
-  const int stages = (a.depth + kDepth - 1) / kDepth;
+// What a product is launched with.
+struct product_call {
+  tensor_args a;
+  CUtensorMap ma, mb;
+  void* out;
+  bool wide, tma;
+  int64_t units;   // no more tiles than that
+};
+
+template <typename T, int MODE, bool TMA>
+cudaError_t launch_product(hpspmm_ctx* ctx, const product_call& c, cudaStream_t s) {
+  if (c.wide) return launch_one<T, MODE, 256, 4, 1, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  const int stages = (c.a.depth + kDepth - 1) / kDepth;
   int cl = 8;
-  while (cl > 1 && (units * cl > ctx->sm_count || stages < 2 * cl)) cl /= 2;
-  if (cl == 8) return launch_one<T, MODE, 64, 7, 8>(ctx, a, ma, mb, out, units, s);
-  if (cl == 4) return launch_one<T, MODE, 64, 7, 4>(ctx, a, ma, mb, out, units, s);
-  if (cl == 2) return launch_one<T, MODE, 64, 7, 2>(ctx, a, ma, mb, out, units, s);
-  return launch_one<T, MODE, 64, 8, 1>(ctx, a, ma, mb, out, units, s);
+  while (cl > 1 && (c.units * cl > ctx->sm_count || stages < 2 * cl)) cl /= 2;
+  if (cl == 8) return launch_one<T, MODE, 64, 7, 8, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (cl == 4) return launch_one<T, MODE, 64, 7, 4, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (cl == 2) return launch_one<T, MODE, 64, 7, 2, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  return launch_one<T, MODE, 64, 8, 1, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+}
+template <typename T>
+cudaError_t launch_product(hpspmm_ctx* ctx, const product_call& c, bool out_first, cudaStream_t s) {
+  if (c.tma)
+    return out_first ? launch_product<T, MODE_OUT_FIRST, true>(ctx, c, s) : launch_product<T, MODE_IN_FIRST, true>(ctx, c, s);
+  return out_first ? launch_product<T, MODE_OUT_FIRST, false>(ctx, c, s) : launch_product<T, MODE_IN_FIRST, false>(ctx, c, s);
+}
+
+template <typename T>
+cudaError_t launch_weight_grad(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* dW, bool tma,
+                               bool wide, int64_t units, cudaStream_t s) {
+  if (tma)
+    return wide ? launch_one<T, MODE_WEIGHT, 256, 4, 1, true>(ctx, a, ma, mb, dW, units, s)
+                : launch_one<T, MODE_WEIGHT, 64, 8, 1, true>(ctx, a, ma, mb, dW, units, s);
+  return wide ? launch_one<T, MODE_WEIGHT, 256, 4, 1, false>(ctx, a, ma, mb, dW, units, s)
+              : launch_one<T, MODE_WEIGHT, 64, 8, 1, false>(ctx, a, ma, mb, dW, units, s);
 }
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-// 0: launched, 1: this path does not take the call, otherwise a status
 int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx,
                                   const void* W, bool out_first, const int32_t* offsets, void* Y, cudaStream_t s) {
-  if (type == HPSPMM_TYPE_F32 || K % 8 || N % 8 || ldx % 8 || ldx < K || !aligned(X) || !aligned(W) || !aligned(Y))
-    return 1;
   const bool half = type == HPSPMM_TYPE_F16;
-  const bool wide = R > 64 * G;
-  const int64_t bn = wide ? 256 : 64;
-  CUtensorMap ma, mb;
+  product_call c = {};
+  const int64_t across = (N + kLanes - 1) / kLanes;
+  // tiles of 256 rows where groups have more than 64 in the mean and the tiles (half a one more for each group) fill the SMs
+  c.wide = R > 64 * G && (R / 256 + G / 2) * across >= ctx->sm_count;
+  c.out = Y;
+  const int64_t bn = c.wide ? 256 : 64;
+  if ((R / bn + G + 1) * across > kMaxTiles || R / bn + G + 1 > kMostTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
   const int64_t wsize[3] = {out_first ? K : N, out_first ? N : K, G}, wstride[2] = {wsize[0], K * N};
   const int wbox[3] = {64, out_first ? kLanes : kDepth, 1};
   const int64_t xsize[2] = {K, R}, xstride[1] = {ldx};
-  const int xbox[2] = {kDepth, wide ? box_rows<256>() : box_rows<64>()};
-  if (!encode(&ma, half, W, 3, wsize, wstride, wbox) || !encode(&mb, half, X, 2, xsize, xstride, xbox)) return 1;
-  const int64_t across = (N + kLanes - 1) / kLanes;
-  if ((R / bn + G + 1) * across > kMaxTiles || R / bn + G + 1 > kMostTiles) return 1;
+  const int xbox[2] = {kDepth, c.wide ? box_rows<256>() : box_rows<64>()};
+  c.tma = K % 8 == 0 && N % 8 == 0 && ldx % 8 == 0 && ldx >= K && aligned(X) && aligned(W) && aligned(Y) &&
+          encode(&c.ma, half, W, 3, wsize, wstride, wbox) && encode(&c.mb, half, X, 2, xsize, xstride, xbox);
   for (int64_t g0 = 0; g0 < G; g0 += kMaxGroups) {
     const int64_t gn = std::min<int64_t>(kMaxGroups, G - g0);
-    const tensor_args a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, {(int)R, 0}, nullptr,
-                           ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
-    const int64_t units = (std::min(R, gn) + R / bn) * across;   // no more than that
-    cudaError_t e;
-    if (half)
-      e = out_first ? launch_product<__half, MODE_OUT_FIRST>(ctx, a, ma, mb, Y, wide, units, s)
-                    : launch_product<__half, MODE_IN_FIRST>(ctx, a, ma, mb, Y, wide, units, s);
-    else
-      e = out_first ? launch_product<__nv_bfloat16, MODE_OUT_FIRST>(ctx, a, ma, mb, Y, wide, units, s)
-                    : launch_product<__nv_bfloat16, MODE_IN_FIRST>(ctx, a, ma, mb, Y, wide, units, s);
-    HPSPMM_CUDA_TRY(ctx, e);
+    c.a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, {(int)R, 0}, nullptr,
+           ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS, W, X, wsize[0], ldx};
+    c.units = (std::min(R, gn) + R / bn) * across;
+    HPSPMM_CUDA_TRY(ctx, half ? launch_product<__half>(ctx, c, out_first, s) : launch_product<__nv_bfloat16>(ctx, c, out_first, s));
   }
   return HPSPMM_OK;
 }
@@ -605,18 +714,20 @@ int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t
 int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t I, int64_t J, int32_t type, const void* A,
                                       int64_t lda, const void* B, int64_t ldb, const int32_t* offsets, void* dW,
                                       const piece_plan& p, float* slots, cudaStream_t s) {
-  if (type == HPSPMM_TYPE_F32 || I % 8 || J % 8 || lda % 8 || ldb % 8 || lda < I || ldb < J || !aligned(A) || !aligned(B))
-    return 1;
   const bool half = type == HPSPMM_TYPE_F16;
-  CUtensorMap ma, mb;   // the operand of the output's columns lies on the lanes
+  const int64_t across = (J + kLanes - 1) / kLanes;
+  const bool wide = (G + p.slots / 2) * ((I + 255) / 256) * across >= ctx->sm_count;   // (about half of the slots are used)
+  const int64_t bn = wide ? 256 : 64, units = (G + p.slots) * ((I + bn - 1) / bn) * across;
+  if (units > kMaxTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
+  CUtensorMap ma = {}, mb = {};   // the operand of the output's columns lies on the lanes
   const int64_t asize[2] = {J, R}, astride[1] = {ldb}, bsize[2] = {I, R}, bstride[1] = {lda};
   const int box[2] = {64, kDepth};
-  if (!encode(&ma, half, B, 2, asize, astride, box) || !encode(&mb, half, A, 2, bsize, bstride, box)) return 1;
-  const int64_t units = (G + p.slots) * ((I + 255) / 256) * ((J + kLanes - 1) / kLanes);
-  if (units > kMaxTiles) return 1;
-  const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, p, slots, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS};
-  const cudaError_t e = half ? launch_one<__half, MODE_WEIGHT, 256, 4, 1>(ctx, a, ma, mb, dW, units, s)
-                             : launch_one<__nv_bfloat16, MODE_WEIGHT, 256, 4, 1>(ctx, a, ma, mb, dW, units, s);
+  const bool tma = I % 8 == 0 && J % 8 == 0 && lda % 8 == 0 && ldb % 8 == 0 && lda >= I && ldb >= J && aligned(A) && aligned(B) &&
+                   encode(&ma, half, B, 2, asize, astride, box) && encode(&mb, half, A, 2, bsize, bstride, box);
+  const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, p, slots, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS,
+                         B, A, ldb, lda};
+  const cudaError_t e = half ? launch_weight_grad<__half>(ctx, a, ma, mb, dW, tma, wide, units, s)
+                             : launch_weight_grad<__nv_bfloat16>(ctx, a, ma, mb, dW, tma, wide, units, s);
   HPSPMM_CUDA_TRY(ctx, e);
   return HPSPMM_OK;
 }
