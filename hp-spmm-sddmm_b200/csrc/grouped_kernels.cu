@@ -23,7 +23,7 @@ struct row_tile {
 };
 
 // The t-th tile of up to `length` rows, of the parts (products) or of the groups (gradients: at least one for each).  Called
-// by one whole warp, which looks at 128 of them at a time.
+// by whole warps, each of which looks at 128 of them at a time.
 template <bool GRADIENT>
 __device__ __forceinline__ row_tile find_row_tile(const int* offsets, int G, int R, int length, int t) {
   const int lane = threadIdx.x & 31, parts = GRADIENT ? G : G + 2;
@@ -82,12 +82,17 @@ __device__ __forceinline__ row_tile find_row_tile(const int* offsets, int G, int
 
 // ---- products on the ordinary cores --------------------------------------------------------------------------------
 //
-// A tile of 128 x BN outputs to a block of 256 threads, 8 x BN / 16 of them to a thread, in 32 bits from the operands on;
-// 16 of the depth at a time through two buffers of shared memory, the next ones on their way to registers meanwhile.
-// Bound by the multiply-adds, two of which go as one packed instruction (fma.rn.f32x2).
+// A tile of TR x BN outputs to a block of 2 TR threads, 8 x BN / 16 of them to a thread, in 32 bits from the operands on;
+// 16 of the depth at a time, copied asynchronously into a ring of three buffers in the order in which they lie in memory.
+// Bound by the multiply-adds, two of which go as one packed instruction (fma.rn.f32x2): on two neighbouring columns of the
+// output, or, where both operands lie along the depth, on two neighbours of it, whose sums meet at the end.
+// TR = 64 for products, whose depth is short as often as not, so that more blocks hide each other's beginnings (100,003 x 100
+// by 47 matrices of 64: 46 us with 128, 41 with 64); 128 for gradients, which read less that way (55 us with 64, 46 with 128).
 
-constexpr int kTileRows = 128;
+constexpr int kProductRows = 64;    // of a tile
+constexpr int kGradientRows = 128;
 constexpr int kTileDepth = 16;
+constexpr int kBuffers = 3;
 
 __device__ __forceinline__ void fma_pair(uint64_t& acc, uint64_t a, uint64_t b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
@@ -97,155 +102,186 @@ __device__ __forceinline__ uint64_t both(float v) {
   asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(v));
   return r;
 }
+__device__ __forceinline__ float half_of(uint64_t v, int h) { return __uint_as_float((uint32_t)(v >> (32 * h))); }
 
-// ROWS x 16 elements of an operand; element (i, k) lies at p[i * stride + k] (ALONG: next to each other along the depth) or
-// p[k * stride + i].  VEC: four neighbours are one aligned load, or none of them is there.
-template <int ROWS, bool ALONG, bool VEC>
-struct tile_loader {
-  static constexpr int kEach = ROWS * kTileDepth / kThreads / 4;   // quads to a thread
-  float v[kEach][4];
-  __device__ __forceinline__ void load(const float* p, int64_t stride, int rows, int depth, int k0) {
+// zeros where `there` is false (nothing is read then)
+template <int BYTES>
+__device__ __forceinline__ void copy_async(float* dst, const float* src, bool there) {
+  const unsigned to = (unsigned)__cvta_generic_to_shared(dst);
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(there ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+
+// ROWS x 16 elements of an operand; element (i, k) lies at p[i * stride + k] (ALONG: next to each other along the depth, and
+// so in the buffer: 20 floats to a row, which keeps the reads of 8 rows off each other's banks) or at p[k * stride + i].
+// VEC: four neighbours are one aligned copy, or none of them is there.
+template <int ROWS, int THREADS, bool ALONG, bool VEC>
+struct operand_tile {
+  static constexpr int kPitch = ALONG ? kTileDepth + 4 : ROWS;
+  static constexpr int kFloats = (ALONG ? ROWS : kTileDepth) * kPitch;
+  static __device__ __forceinline__ void copy(float* s, const float* p, int64_t stride, int rows, int depth, int k0) {
 #pragma unroll
-    for (int u = 0; u < kEach; ++u) {
-      const int q = threadIdx.x + u * kThreads;
-      const int i = ALONG ? q >> 2 : q % (ROWS / 4) * 4, k = k0 + (ALONG ? (q & 3) * 4 : q / (ROWS / 4));
+    for (int u = 0; u < ROWS * kTileDepth / THREADS / 4; ++u) {
+      const int q = threadIdx.x + u * THREADS;
+      const int line = ALONG ? q >> 2 : q / (ROWS / 4), in = (ALONG ? q & 3 : q % (ROWS / 4)) * 4;
+      const int i = ALONG ? line : in, k = k0 + (ALONG ? in : line);
+      const int left = ALONG ? (i < rows ? depth - k : 0) : (k < depth ? rows - i : 0);
       const float* at = p + (ALONG ? i * stride + k : k * stride + i);
-      const bool line = ALONG ? i < rows : k < depth;
-      const int left = !line ? 0 : (ALONG ? depth - k : rows - i);
+      float* to = s + line * kPitch + in;
       if (VEC) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (left > 0) x = __ldg(reinterpret_cast<const float4*>(at));
-        v[u][0] = x.x, v[u][1] = x.y, v[u][2] = x.z, v[u][3] = x.w;
+        copy_async<16>(to, left > 0 ? at : p, left > 0);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[u][e] = e < left ? __ldg(at + e) : 0.f;
-      }
-    }
-  }
-  __device__ __forceinline__ void store(float (*s)[ROWS + 4]) const {
-#pragma unroll
-    for (int u = 0; u < kEach; ++u) {
-      const int q = threadIdx.x + u * kThreads;
-      if (ALONG) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[(q & 3) * 4 + e][q >> 2] = v[u][e];
-      } else {
-        *reinterpret_cast<float4*>(&s[q / (ROWS / 4)][q % (ROWS / 4) * 4]) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+        for (int e = 0; e < 4; ++e) copy_async<4>(to + e, e < left ? at + e : p, e < left);
       }
     }
   }
 };
 
+template <int TR, int BN, bool A_ALONG, bool B_ALONG, bool VEC>
+struct tile_shape {
+  typedef operand_tile<TR, 2 * TR, A_ALONG, VEC> a;
+  typedef operand_tile<BN, 2 * TR, B_ALONG, VEC> b;
+  static constexpr int kBytes = kBuffers * (a::kFloats + b::kFloats) * 4;
+};
+
 // C[i][j] = sum over k < depth of A(i, k) * B(k, j) for i < rows, j < cols.
-template <int BN, bool A_ALONG, bool B_ALONG, bool VEC>
+template <int TR, int BN, bool A_ALONG, bool B_ALONG, bool VEC>
 __device__ __forceinline__ void tile_product(const float* A, int64_t sa, const float* B, int64_t sb, int rows, int cols, int depth, float* C,
-                                             int64_t sc, float (*As)[kTileDepth][kTileRows + 4], float (*Bs)[kTileDepth][BN + 4]) {
-  constexpr int kHalves = BN / 64;
+                                             int64_t sc, float* smem) {
+  typedef tile_shape<TR, BN, A_ALONG, B_ALONG, VEC> shape;
+  typedef typename shape::a ta;
+  typedef typename shape::b tb;
+  static_assert(!B_ALONG || (A_ALONG && BN == 64), "two along the depth take twice the accumulators");
+  constexpr bool kDeep = A_ALONG && B_ALONG;
+  constexpr int kHalves = BN / 64, kAcc = kDeep ? 4 : 2 * kHalves;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  uint64_t acc[8][kHalves * 2];
+  auto row_of = [&](int x) { return ty * 4 + (x & 3) + (x >> 2) * (TR / 2); };
+  float* const bs = smem + kBuffers * ta::kFloats;
+  const int steps = (depth + kTileDepth - 1) / kTileDepth;
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      ta::copy(smem + step % kBuffers * ta::kFloats, A, sa, rows, depth, step * kTileDepth);
+      tb::copy(bs + step % kBuffers * tb::kFloats, B, sb, cols, depth, step * kTileDepth);
+    }
+    cp_async_commit();
+  };
+  uint64_t acc[8][kAcc];
 #pragma unroll
   for (int x = 0; x < 8; ++x)
 #pragma unroll
-    for (int y = 0; y < kHalves * 2; ++y) acc[x][y] = 0;
-  tile_loader<kTileRows, A_ALONG, VEC> la;
-  tile_loader<BN, B_ALONG, VEC> lb;
-  la.load(A, sa, rows, depth, 0), lb.load(B, sb, cols, depth, 0);
-  la.store(As[0]), lb.store(Bs[0]);
-  __syncthreads();
-  int buf = 0;
-  for (int k0 = 0; k0 < depth; k0 += kTileDepth) {
-    const bool more = k0 + kTileDepth < depth;
-    if (more) la.load(A, sa, rows, depth, k0 + kTileDepth), lb.load(B, sb, cols, depth, k0 + kTileDepth);
+    for (int y = 0; y < kAcc; ++y) acc[x][y] = 0;
 #pragma unroll
-    for (int k = 0; k < kTileDepth; ++k) {
-      float a[8];
-      uint64_t b[kHalves * 2];
+  for (int i = 0; i < kBuffers - 1; ++i) fetch(i);
+  for (int step = 0; step < steps; ++step) {
+    cp_async_wait<kBuffers - 2>();
+    __syncthreads();
+    fetch(step + kBuffers - 1);      // into the buffer that everybody has left
+    const float *as = smem + step % kBuffers * ta::kFloats, *b0 = bs + step % kBuffers * tb::kFloats;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(a + 4 * h) = *reinterpret_cast<const float4*>(&As[buf][k][ty * 4 + 64 * h]);
+    for (int k = 0; k < kTileDepth; k += 4) {
+      if (kDeep) {
+        ulonglong2 a[8], b[4];
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h)
-        *reinterpret_cast<ulonglong2*>(b + 2 * h) = *reinterpret_cast<const ulonglong2*>(&Bs[buf][k][tx * 4 + 64 * h]);
+        for (int x = 0; x < 8; ++x) a[x] = *reinterpret_cast<const ulonglong2*>(as + row_of(x) * ta::kPitch + k);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const uint64_t aa = both(a[x]);
+        for (int y = 0; y < 4; ++y) b[y] = *reinterpret_cast<const ulonglong2*>(b0 + (tx + 16 * y) * tb::kPitch + k);
 #pragma unroll
-        for (int y = 0; y < kHalves * 2; ++y) fma_pair(acc[x][y], aa, b[y]);
+        for (int x = 0; x < 8; ++x)
+#pragma unroll
+          for (int y = 0; y < kAcc; ++y) fma_pair(acc[x][y], a[x].x, b[y % 4].x), fma_pair(acc[x][y], a[x].y, b[y % 4].y);
+      } else {
+        float a[4][8];   // [k][x]
+        if (A_ALONG) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float4 v = *reinterpret_cast<const float4*>(as + row_of(x) * ta::kPitch + k);
+            a[0][x] = v.x, a[1][x] = v.y, a[2][x] = v.z, a[3][x] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              *reinterpret_cast<float4*>(&a[i][4 * h]) = *reinterpret_cast<const float4*>(as + (k + i) * ta::kPitch + ty * 4 + TR / 2 * h);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint64_t b[2 * kHalves];
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            *reinterpret_cast<ulonglong2*>(b + 2 * h) = *reinterpret_cast<const ulonglong2*>(b0 + (k + i) * tb::kPitch + tx * 4 + 64 * h);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const uint64_t aa = both(a[i][x]);
+#pragma unroll
+            for (int y = 0; y < 2 * kHalves; ++y) fma_pair(acc[x][y % kAcc], aa, b[y]);
+          }
+        }
       }
-    }
-    if (more) {
-      la.store(As[buf ^ 1]), lb.store(Bs[buf ^ 1]);
-      __syncthreads();
-      buf ^= 1;
     }
   }
 #pragma unroll
   for (int x = 0; x < 8; ++x) {
-    const int i = ty * 4 + (x & 3) + (x >> 2) * 64;
-    if (i >= rows) continue;
+    if (row_of(x) >= rows) continue;
+    float* to = C + (int64_t)row_of(x) * sc;
+    if (kDeep) {
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const int j = tx * 4 + 64 * h;
-      float* to = C + (int64_t)i * sc + j;
-      float v[4];
+      for (int y = 0; y < 4; ++y)
+        if (tx + 16 * y < cols) to[tx + 16 * y] = half_of(acc[x][y % kAcc], 0) + half_of(acc[x][y % kAcc], 1);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        v[2 * e] = __uint_as_float((uint32_t)acc[x][2 * h + e]);
-        v[2 * e + 1] = __uint_as_float((uint32_t)(acc[x][2 * h + e] >> 32));
-      }
-      if (VEC) {
-        if (j < cols) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-      } else {
+      for (int h = 0; h < kHalves; ++h) {
+        const int j = tx * 4 + 64 * h;
+        const float v[4] = {half_of(acc[x][2 * h % kAcc], 0), half_of(acc[x][2 * h % kAcc], 1), half_of(acc[x][(2 * h + 1) % kAcc], 0),
+                            half_of(acc[x][(2 * h + 1) % kAcc], 1)};
+        if (VEC) {
+          if (j < cols) *reinterpret_cast<float4*>(to + j) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j + e < cols) to[e] = v[e];
+          for (int e = 0; e < 4; ++e)
+            if (j + e < cols) to[j + e] = v[e];
+        }
       }
     }
   }
 }
 
 template <int BN, bool OUT_FIRST, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(2 * kProductRows, BN == 64 && !OUT_FIRST ? 5 : 4)
 grouped_product_kernel(int R, int G, int K, int N, const float* __restrict__ X, int64_t ldx, const float* __restrict__ W, const int* offsets,
                        float* __restrict__ Y, int col_tiles) {
-  __shared__ float As[2][kTileDepth][kTileRows + 4], Bs[2][kTileDepth][BN + 4];
-  __shared__ row_tile shared_tile;
+  extern __shared__ float4 tile_smem[];
   const int t = blockIdx.x / col_tiles, j0 = (blockIdx.x - t * col_tiles) * BN;
-  if (threadIdx.x < 32) {
-    const row_tile found = find_row_tile<false>(offsets, G, R, kTileRows, t);
-    if (threadIdx.x == 0) shared_tile = found;
-  }
-  __syncthreads();
-  const row_tile w = shared_tile;
+  const row_tile w = find_row_tile<false>(offsets, G, R, kProductRows, t);
   if (w.rows == 0) return;
   const bool none = w.g >= G;
   const float* wg = none ? W : W + (int64_t)w.g * K * N;
-  tile_product<BN, true, OUT_FIRST, VEC>(X + (int64_t)w.r0 * ldx, ldx, OUT_FIRST ? wg + (int64_t)j0 * K : wg + j0, OUT_FIRST ? K : N,
-                                               w.rows, min(BN, N - j0), none ? 0 : K, Y + (int64_t)w.r0 * N + j0, N, As, Bs);
+  tile_product<kProductRows, BN, true, OUT_FIRST, VEC>(X + (int64_t)w.r0 * ldx, ldx, OUT_FIRST ? wg + (int64_t)j0 * K : wg + j0, OUT_FIRST ? K : N,
+                                               w.rows, min(BN, N - j0), none ? 0 : K, Y + (int64_t)w.r0 * N + j0, N,
+                                         reinterpret_cast<float*>(tile_smem));
 }
 
 // dW[g][i][j] = sum over the rows of the group of A[r][i] * B[r][j]
 template <int BN, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(2 * kGradientRows, 2)
 grouped_weight_grad_kernel(int R, int G, int I, int J, const float* __restrict__ A, int64_t lda, const float* __restrict__ B, int64_t ldb,
                            const int* offsets, float* __restrict__ dW, const piece_plan plan, float* slots, int i_tiles, int j_tiles) {
-  __shared__ float As[2][kTileDepth][kTileRows + 4], Bs[2][kTileDepth][BN + 4];
-  __shared__ row_tile shared_tile;
+  extern __shared__ float4 tile_smem[];
   int t = blockIdx.x;
   const int j0 = t % j_tiles * BN;
   t /= j_tiles;
-  const int i0 = t % i_tiles * kTileRows;
+  const int i0 = t % i_tiles * kGradientRows;
   t /= i_tiles;
-  if (threadIdx.x < 32) {
-    const row_tile found = find_row_tile<true>(offsets, G, R, plan.length, t);
-    if (threadIdx.x == 0) shared_tile = found;
-  }
-  __syncthreads();
-  const row_tile w = shared_tile;
+  const row_tile w = find_row_tile<true>(offsets, G, R, plan.length, t);
   if (w.pieces == 0 || (w.pieces > 1 && w.slot >= plan.slots)) return;
   const float *a = A + (int64_t)w.r0 * lda + i0, *b = B + (int64_t)w.r0 * ldb + j0;
-  const int rows = min(kTileRows, I - i0), cols = min(BN, J - j0);
+  const int rows = min(kGradientRows, I - i0), cols = min(BN, J - j0);
   float* to = w.pieces == 1 ? dW + (int64_t)w.g * I * J : slots + (int64_t)w.slot * I * J;
-  tile_product<BN, false, false, VEC>(a, lda, b, ldb, rows, cols, w.rows, to + (int64_t)i0 * J + j0, J, As, Bs);
+  tile_product<kGradientRows, BN, false, false, VEC>(a, lda, b, ldb, rows, cols, w.rows, to + (int64_t)i0 * J + j0, J,
+                                      reinterpret_cast<float*>(tile_smem));
 }
 
 // Groups of more than one piece: the pieces in order.
@@ -280,22 +316,26 @@ join_pieces_kernel(int R, int G, int64_t elements, const int* offsets, const pie
   }
 }
 
+// (a refused size of the shared memory shows at the launch)
 template <int BN, bool OUT_FIRST, bool VEC>
 void launch_product(int64_t R, int64_t G, int64_t K, int64_t N, const void* X, int64_t ldx, const void* W, const int32_t* offsets,
                     void* Y, cudaStream_t s) {
-  const int64_t col_tiles = (N + BN - 1) / BN, blocks = ((R + kTileRows - 1) / kTileRows + G + 2) * col_tiles;
-  grouped_product_kernel<BN, OUT_FIRST, VEC><<<(unsigned)blocks, kThreads, 0, s>>>((int)R, (int)G, (int)K, (int)N, (const float*)X, ldx,
-                                                                                  (const float*)W, offsets, (float*)Y, (int)col_tiles);
+  constexpr int smem = tile_shape<kProductRows, BN, true, OUT_FIRST, VEC>::kBytes;
+  cudaFuncSetAttribute(grouped_product_kernel<BN, OUT_FIRST, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int64_t col_tiles = (N + BN - 1) / BN, blocks = ((R + kProductRows - 1) / kProductRows + G + 2) * col_tiles;
+  grouped_product_kernel<BN, OUT_FIRST, VEC><<<(unsigned)blocks, 2 * kProductRows, smem, s>>>(
+      (int)R, (int)G, (int)K, (int)N, (const float*)X, ldx, (const float*)W, offsets, (float*)Y, (int)col_tiles);
 }
 
 template <int BN, bool VEC>
 void launch_weight_grad(int64_t R, int64_t G, int64_t I, int64_t J, const void* A, int64_t lda, const void* B, int64_t ldb,
                         const int32_t* offsets, void* dW, const piece_plan& p, float* slots, cudaStream_t s) {
-  const int64_t i_tiles = (I + kTileRows - 1) / kTileRows, j_tiles = (J + BN - 1) / BN;
+  constexpr int smem = tile_shape<kGradientRows, BN, false, false, VEC>::kBytes;
+  cudaFuncSetAttribute(grouped_weight_grad_kernel<BN, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int64_t i_tiles = (I + kGradientRows - 1) / kGradientRows, j_tiles = (J + BN - 1) / BN;
   const int64_t blocks = (G + piece_slots(R, p.length)) * i_tiles * j_tiles;
-  grouped_weight_grad_kernel<BN, VEC><<<(unsigned)blocks, kThreads, 0, s>>>((int)R, (int)G, (int)I, (int)J, (const float*)A, lda,
-                                                                           (const float*)B, ldb, offsets, (float*)dW, p, slots, (int)i_tiles,
-                                                                              (int)j_tiles);
+  grouped_weight_grad_kernel<BN, VEC><<<(unsigned)blocks, 2 * kGradientRows, smem, s>>>(
+      (int)R, (int)G, (int)I, (int)J, (const float*)A, lda, (const float*)B, ldb, offsets, (float*)dW, p, slots, (int)i_tiles, (int)j_tiles);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -308,7 +348,7 @@ int64_t tile_columns(int64_t cols) { return cols <= 64 ? 64 : 128; }
 // tile in 32 bits).  All the rows where there are tiles enough.
 piece_plan plan_pieces(int64_t R, int64_t G, int64_t I, int64_t J, int32_t type) {
   const bool f32 = type == HPSPMM_TYPE_F32;
-  const int64_t bi = f32 ? kTileRows : 256, bj = f32 ? tile_columns(J) : 128;
+  const int64_t bi = f32 ? kGradientRows : 256, bj = f32 ? tile_columns(J) : 128;
   const int64_t tiles = ((I + bi - 1) / bi) * ((J + bj - 1) / bj), target = 148 * (f32 ? 4 : 2);
   int64_t length = R;
   if (tiles < target && G <= kMostSplitGroups) length = std::max<int64_t>(f32 ? 256 : 1024, (R * tiles / target + 63) / 64 * 64);
@@ -340,15 +380,6 @@ int hpspmm_join_pieces(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t elements, 
   return HPSPMM_OK;
 }
 
-template <int BN, bool VEC>
-void launch_product(bool out_first, int64_t R, int64_t G, int64_t K, int64_t N, const void* X, int64_t ldx, const void* W,
-                    const int32_t* offsets, void* Y, cudaStream_t s) {
-  if (out_first)
-    launch_product<BN, true, VEC>(R, G, K, N, X, ldx, W, offsets, Y, s);
-  else
-    launch_product<BN, false, VEC>(R, G, K, N, X, ldx, W, offsets, Y, s);
-}
-
 extern "C" {
 
 int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type, const void* X,
@@ -369,18 +400,22 @@ int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int
   }
   if (type != HPSPMM_TYPE_F32)
     return hpspmm_grouped_product_tensor(ctx, R, G, K, N, type, X, ldx, W, w_out_first != 0, offsets, Y, s);
-  if (((R + kTileRows - 1) / kTileRows + G + 2) * ((N + 63) / 64) > 2147483647ll)
-    return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 128 x 64");
+  if (((R + kProductRows - 1) / kProductRows + G + 2) * ((N + 63) / 64) > 2147483647ll)
+    return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 64 x 64");
   const bool vec = K % 4 == 0 && N % 4 == 0 && ldx % 4 == 0 && aligned16(X) && aligned16(W) && aligned16(Y);
   const bool narrow = tile_columns(N) == 64, of = w_out_first != 0;
-  if (vec && narrow)
-    launch_product<64, true>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+  if (of && vec)
+    launch_product<64, true, true>(R, G, K, N, X, ldx, W, offsets, Y, s);
+  else if (of)
+    launch_product<64, true, false>(R, G, K, N, X, ldx, W, offsets, Y, s);
+  else if (vec && narrow)
+    launch_product<64, false, true>(R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (vec)
-    launch_product<128, true>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<128, false, true>(R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (narrow)
-    launch_product<64, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<64, false, false>(R, G, K, N, X, ldx, W, offsets, Y, s);
   else
-    launch_product<128, false>(of, R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<128, false, false>(R, G, K, N, X, ldx, W, offsets, Y, s);
   ctx->launches++;
   HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
   return HPSPMM_OK;
@@ -422,7 +457,7 @@ int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K,
     const int done = hpspmm_grouped_weight_grad_tensor(ctx, R, G, I, J, type, A, lda, B, ldb, offsets, dW, p, slots, s);
     if (done != HPSPMM_OK) return done;
   } else {
-    if ((G + p.slots) * ((I + kTileRows - 1) / kTileRows) * ((J + 63) / 64) > 2147483647ll)
+    if ((G + p.slots) * ((I + kGradientRows - 1) / kGradientRows) * ((J + 63) / 64) > 2147483647ll)
       return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 128 x 64");
     const bool vec = I % 4 == 0 && J % 4 == 0 && lda % 4 == 0 && ldb % 4 == 0 && aligned16(A) && aligned16(B) &&
                      aligned16(dW);
