@@ -95,13 +95,29 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return mbar_try<CLUSTER>(bar, parity) || mbar_wait_slow<CLUSTER>(bar, parity, failed);
 }
 
+// PAIR: the barrier may be the one of the pair's other block (`bar` is an address in the cluster's window)
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-               "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-               "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+  if (PAIR)
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
 }
 
 // Shared-memory operand, 128-byte swizzle.  Along the depth (LINES_OF_DEPTH: every 128-byte line holds 64 elements along
@@ -116,12 +132,40 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr) {
 template <bool LINES_OF_DEPTH>
 __device__ __forceinline__ constexpr uint64_t operand_step() { return LINES_OF_DEPTH ? 32 >> 4 : (16 * 128) >> 4; }
 
+template <bool PAIR>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a),
-               "l"(b), "r"(instr), "r"((int)add) : "memory");
+  if (PAIR)
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(instr), "r"((int)add) : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(instr), "r"((int)add) : "memory");
 }
+// arrives (in a pair: at both blocks' barrier of that place) once the products issued so far are done
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+template <bool PAIR, int COLUMNS>
+__device__ __forceinline__ void tensor_alloc(uint32_t to) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "n"(COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "n"(COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <bool PAIR, int COLUMNS>
+__device__ __forceinline__ void tensor_free(uint32_t base) {
+  if (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS) : "memory");
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS) : "memory");
 }
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -150,20 +194,22 @@ struct tile {
   int slot;            // gradients: where a piece of a group goes, -1: to the matrix itself
 };
 
-template <int MODE, int BN, int CL>
+// WIDTH: columns of the output to a tile (128, of a pair of blocks 256)
+template <int MODE, int BN, int WIDTH>
 __device__ __forceinline__ int tile_count(const tensor_args& a, const int* ends) {
-  const int across = (a.cols + kLanes - 1) / kLanes;
+  const int across = (a.cols + WIDTH - 1) / WIDTH;
   if (MODE == MODE_WEIGHT)
     return (int)min((int64_t)(a.plan.slots ? ends[a.gn - 1] : a.gn) * ((a.rows + BN - 1) / BN) * across, (int64_t)kMaxTiles);
   return (int)min((int64_t)ends[a.gn - 1] * across, (int64_t)kMaxTiles);
 }
 
-template <int MODE, int BN, int CL>
+template <int MODE, int BN, int CL, bool PAIR>
 __device__ __forceinline__ tile tile_at(const tensor_args& a, const int* ends, const int* slot_ends, int u, int rank) {
   tile t;
-  const int across = (a.cols + kLanes - 1) / kLanes;
+  constexpr int kWidth = PAIR ? 2 * kLanes : kLanes;
+  const int across = (a.cols + kWidth - 1) / kWidth;
   int q = u / across;
-  t.col0 = (u - q * across) * kLanes;
+  t.col0 = (u - q * across) * kWidth + (PAIR ? rank * kLanes : 0);
   t.slot = -1;
   if (MODE == MODE_WEIGHT) {
     const int down = (a.rows + BN - 1) / BN;
@@ -205,6 +251,12 @@ __device__ __forceinline__ tile tile_at(const tensor_args& a, const int* ends, c
   t.end = CL == 1 ? stages : (int)((int64_t)stages * (rank + 1) / CL);
   t.stages = t.end - t.begin;
   return t;
+}
+
+// Whether a stage of a gradient ends inside the instruction's depth of 16: the rows behind belong to the next group.
+__device__ __forceinline__ bool cut_short(const tile& t, int stage) {
+  const int left = t.end - t.begin - stage * kDepth;
+  return left < kDepth && (left & 15);
 }
 
 template <typename T>
@@ -266,22 +318,25 @@ __device__ __forceinline__ void load_lines(const uint16_t* p, int64_t ld, int wa
   }
 }
 
-template <int BN, int STAGES, int CL>
-constexpr int smem_bytes() { return 1024 + STAGES * (kABytes + BN * 128) + (CL > 1 ? BN * kLanes * 4 : 0); }
+template <int BN, int STAGES, int CL, bool PAIR>
+constexpr int smem_bytes() { return 1024 + STAGES * (kABytes + BN * 128 / (PAIR ? 2 : 1)) + (CL > 1 ? BN * kLanes * 4 : 0); }
 
-template <typename T, int MODE, int BN, int STAGES, int CL, bool TMA>
+template <typename T, int MODE, int BN, int STAGES, int CL, bool TMA, bool PAIR>
 __global__ void __launch_bounds__(TMA ? kThreads : kThreads + kTeams * kLoaders * 32, 1)
 grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                       T* __restrict__ out) {
   constexpr bool kWeight = MODE == MODE_WEIGHT;
   constexpr bool kALines = MODE == MODE_OUT_FIRST, kBLines = !kWeight;   // which operands have lines along the depth
-  constexpr int kBBytes = BN * 128, kStage = kABytes + kBBytes, kBox = box_rows<BN>();
+  constexpr int kBlocks = PAIR ? 2 : CL;                                 // of a cluster
+  static_assert(!PAIR || (CL == 1 && TMA), "pairs neither split the depth nor go without TMA");
+  // of the N side, a block of a pair holds one half
+  constexpr int kBBytes = BN * 128 / (PAIR ? 2 : 1), kStage = kABytes + kBBytes, kBox = box_rows<BN>();
   constexpr int kColumns = 2 * BN < 32 ? 32 : 2 * BN;                   // of tensor memory: two accumulators
   extern __shared__ char raw[];
   __shared__ int ends[kMaxGroups];
   __shared__ int slot_ends[kWeight ? kMaxGroups : 1];
   __shared__ int part[kThreads / 32];
-  __shared__ uint64_t bars[2 * STAGES + 6];
+  __shared__ uint64_t bars[4 * STAGES + 6];
   __shared__ uint32_t tmem_base;
   __shared__ int failed;
   const uint32_t base = (smem_of(raw) + 1023) / 1024 * 1024;
@@ -290,16 +345,18 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
   auto acc_empty = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
+  auto cut_full = [&](int s) { return bar0 + 8u * (3 * STAGES + 6 + s); };  // a stage that is cut short has been copied
+  auto cleared = [&](int s) { return bar0 + 8u * (2 * STAGES + 6 + s); };   // and has its zeros
   const uint32_t parts_full = bar0 + 8u * (2 * STAGES + 4), parts_empty = bar0 + 8u * (2 * STAGES + 5);
   float* const parts = reinterpret_cast<float*>(raw + (base - smem_of(raw)) + STAGES * kStage);   // [source][row][lane]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int rank = 0;
-  if (CL > 1) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  if (kBlocks > 1) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
 
   if (threadIdx.x == 0) {
     failed = 0;
-    for (int s = 0; s < STAGES; ++s) mbar_init(full(s), TMA ? 1 : kLoaders), mbar_init(empty(s), 1);
-    for (int b = 0; b < 2; ++b) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 4);
+    for (int s = 0; s < STAGES; ++s) mbar_init(full(s), TMA ? 1 : kLoaders), mbar_init(empty(s), 1), mbar_init(cleared(s), PAIR ? 2 : 1), mbar_init(cut_full(s), 1);
+    for (int b = 0; b < 2; ++b) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), PAIR ? 8 : 4);
     mbar_init(parts_full, 4 * CL), mbar_init(parts_empty, 4 * CL);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (TMA) {
@@ -308,8 +365,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     }
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(&tmem_base)), "n"(kColumns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tensor_alloc<PAIR, kColumns>(smem_of(&tmem_base));
     tensor_fence_before();
   }
   chain_grid();
@@ -354,14 +410,14 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   if (!kWeight || a.plan.slots) prefix(ends, false);
   if (kWeight && a.plan.slots) prefix(slot_ends, true);
   __syncthreads();
-  if (CL > 1) {   // the others' barriers are ready
+  if (kBlocks > 1) {   // the others' barriers are ready
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   tensor_fence_after();
   const uint32_t tmem = tmem_base;
-  const int units = tile_count<MODE, BN, CL>(a, ends);
-  const int first = blockIdx.x / CL, step = gridDim.x / CL;
+  const int units = tile_count<MODE, BN, PAIR ? 2 * kLanes : kLanes>(a, ends);
+  const int first = blockIdx.x / kBlocks, step = gridDim.x / kBlocks;
 
   if (warp == 0) {
     if (TMA && lane == 0) {   // copies
@@ -369,89 +425,130 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       uint32_t phase = 0;
       bool ok = true;
       for (int u = first; u < units && ok; u += step) {
-        const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
-        const int boxes = (t.rows + kBox - 1) / kBox;
+        const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
+        // of the N side, this block's part: rows [from, from + count)
+        const int half = (t.rows + 31) / 32 * 16;
+        const int from = t.row0 + (PAIR ? rank * half : 0), count = PAIR ? half : t.rows;
+        const int boxes = (count + kBox - 1) / kBox;
         for (int k = 0; k < t.stages; ++k) {
           ok = mbar_wait(empty(s), phase ^ 1, &failed);
           if (!ok) break;
-          const uint32_t dst = base + s * kStage, bar = full(s);
+          // The copies of both blocks of a pair arrive at the first one's barrier.  A stage that is cut short has a barrier of
+          // its own, in either block: its rest has to be cleared before it is used.
+          const bool cut = kWeight && cut_short(t, k), shared = PAIR && !cut;
+          const uint32_t dst = base + s * kStage, own = cut ? cut_full(s) : full(s), bar = shared ? in_block(own, 0) : own;
+          const uint32_t bytes = kABytes + (kWeight ? (count + 63) / 64 * 8192 : boxes * kBox * 128);
+          if (!shared || rank == 0) mbar_expect(own, shared ? 2 * bytes : bytes);
           if (kWeight) {
-            const int wide = (t.rows + 63) / 64, r = t.begin + k * kDepth;
-            mbar_expect(bar, kABytes + wide * 8192);
-            tma_load(dst, &map_a, bar, t.col0, r);
-            tma_load(dst + 8192, &map_a, bar, t.col0 + 64, r);
-            for (int b = 0; b < wide; ++b) tma_load(dst + kABytes + b * 8192, &map_b, bar, t.row0 + b * 64, r);
+            const int wide = (count + 63) / 64, r = t.begin + k * kDepth;
+            tma_load<PAIR>(dst, &map_a, bar, t.col0, r);
+            tma_load<PAIR>(dst + 8192, &map_a, bar, t.col0 + 64, r);
+            for (int b = 0; b < wide; ++b) tma_load<PAIR>(dst + kABytes + b * 8192, &map_b, bar, from + b * 64, r);
           } else {
             const int d = (t.begin + k) * kDepth;
-            mbar_expect(bar, kABytes + boxes * kBox * 128);
             if (MODE == MODE_OUT_FIRST) {
-              tma_load(dst, &map_a, bar, d, t.col0, t.g);
+              tma_load<PAIR>(dst, &map_a, bar, d, t.col0, t.g);
             } else {
-              tma_load(dst, &map_a, bar, t.col0, d, t.g);
-              tma_load(dst + 8192, &map_a, bar, t.col0 + 64, d, t.g);
+              tma_load<PAIR>(dst, &map_a, bar, t.col0, d, t.g);
+              tma_load<PAIR>(dst + 8192, &map_a, bar, t.col0 + 64, d, t.g);
             }
-            for (int b = 0; b < boxes; ++b) tma_load(dst + kABytes + b * kBox * 128, &map_b, bar, d, t.row0 + b * kBox);
+            for (int b = 0; b < boxes; ++b) tma_load<PAIR>(dst + kABytes + b * kBox * 128, &map_b, bar, d, from + b * kBox);
           }
           if (++s == STAGES) s = 0, phase ^= 1;
         }
       }
     }
     __syncwarp();
-  } else if (warp == 1) {   // products
-    int s = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    for (int u = first; u < units; u += step) {
-      const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
-      if (!mbar_wait(acc_empty(acc), acc_phase ^ 1, &failed)) break;
-      tensor_fence_after();
-      const uint32_t d = tmem + acc * BN;
-      const int n = (t.rows + 15) / 16 * 16;
-      // accumulate in 32 bits; type of A and B; whether their lines run across the depth; N / 8; M / 16
-      const uint32_t instr = 1u << 4 | type_code<T>::value << 7 | type_code<T>::value << 10 | (uint32_t)!kALines << 15 |
-                             (uint32_t)!kBLines << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(kLanes >> 4) << 24;
+  } else if (warp == 1) {
+    // Products, by one thread (of a pair: the first block's).  The next instruction has to be there when the one before it
+    // ends, 128 cycles later: with the whole warp on its way through the loop and the next tile looked up between two of them
+    // the tensor cores stood still for a third of the time.
+    if (lane == 0 && !(PAIR && rank)) {
+      struct {
+        int stages, rows, steps;   // steps: of 16 of the depth, in the last stage
+        bool cut;
+      } w, next = {};
+      auto look_up = [&](int u) {
+        if (u >= units) return;
+        const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
+        const int left = (kWeight ? t.end - t.begin : a.depth - t.begin * kDepth) - (t.stages - 1) * kDepth;
+        next.stages = t.stages, next.rows = t.rows, next.steps = min(kDepth / 16, (left + 15) / 16);
+        next.cut = kWeight && TMA && t.stages > 0 && cut_short(t, t.stages - 1);
+      };
+      const uint64_t first_a = operand<kALines>(base), first_b = operand<kBLines>(base + kABytes);
+      int s = 0, acc = 0;
+      uint32_t acc_phase = 0, full_phase = 0, cut_phase = 0;   // a bit for each stage, which has two barriers
       bool ok = true;
-      for (int k = 0; k < t.stages; ++k) {
-        ok = mbar_wait(full(s), phase, &failed);
+      look_up(first);
+      for (int u = first; u < units && ok; u += step) {
+        w = next;
+        ok = mbar_wait<PAIR>(acc_empty(acc), acc_phase ^ 1, &failed);
         if (!ok) break;
         tensor_fence_after();
-        const uint32_t src = base + s * kStage;
-        int left;   // of the depth in this stage
-        if (kWeight) {
-          left = t.end - t.begin - k * kDepth;
-          if (TMA && left < kDepth && (left & 15)) {   // the next group's rows, up to the end of the instruction's depth, become zeros
-            const int wide = 2 + (t.rows + 63) / 64, rows = 16 - (left & 15);
-            for (int i = lane; i < wide * rows * 8; i += 32) {
-              const int b = i / (rows * 8), r = left + (i >> 3) % rows;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(src + b * 8192 + r * 128 + (i & 7) * 16), "r"(0) : "memory");
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+        const uint32_t d = tmem + acc * BN;
+        const int n = PAIR ? (w.rows + 31) / 32 * 32 : (w.rows + 15) / 16 * 16;
+        // accumulate in 32 bits; type of A and B; whether their lines run across the depth; N / 8; M / 16
+        const uint32_t instr = 1u << 4 | type_code<T>::value << 7 | type_code<T>::value << 10 | (uint32_t)!kALines << 15 |
+                               (uint32_t)!kBLines << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)((PAIR ? 2 : 1) * kLanes >> 4) << 24;
+        for (int k = 0; k < w.stages; ++k) {
+          const bool last = k + 1 == w.stages;
+          if (last && w.cut) {
+            ok = mbar_wait<PAIR>(cleared(s), cut_phase >> s & 1, &failed);
+            cut_phase ^= 1u << s;
+          } else {
+            ok = mbar_wait(full(s), full_phase >> s & 1, &failed);
+            full_phase ^= 1u << s;
           }
-        } else {
-          left = a.depth - (t.begin + k) * kDepth;
+          if (!ok) break;
+          tensor_fence_after();
+          const uint64_t da = first_a + (uint64_t)(s * (kStage >> 4)), db = first_b + (uint64_t)(s * (kStage >> 4));
+          const int steps = last ? w.steps : kDepth / 16;
+          mma<PAIR>(d, da, db, instr, k > 0);
+#pragma unroll
+          for (int i = 1; i < kDepth / 16; ++i)
+            if (i < steps) mma<PAIR>(d, da + i * operand_step<kALines>(), db + i * operand_step<kBLines>(), instr, true);
+          mma_commit<PAIR>(empty(s));
+          if (k == 0) look_up(u + step);
+          if (++s == STAGES) s = 0;
         }
+        if (!ok) break;
+        if (w.stages) {
+          mma_commit<PAIR>(acc_full(acc));
+        } else {
+          look_up(u + step);
+          mbar_arrive(acc_full(acc));
+          if (PAIR) mbar_arrive_remote(acc_full(acc), 1);
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (kWeight && TMA && warp == 3) {   // the rows behind a group, up to the end of the instruction's depth, become zeros
+    int s = 0;
+    uint32_t phase = 0;   // a bit for each stage
+    for (int u = first; u < units; u += step) {
+      const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
+      if (t.stages == 0) continue;
+      s = (s + t.stages - 1) % STAGES;
+      if (cut_short(t, t.stages - 1)) {
+        if (!mbar_wait(cut_full(s), phase >> s & 1, &failed)) break;
+        phase ^= 1u << s;
+        const uint32_t src = base + s * kStage;
+        const int left = t.end - t.begin - (t.stages - 1) * kDepth;
+        const int wide = 2 + ((PAIR ? (t.rows + 31) / 32 * 16 : t.rows) + 63) / 64, rows = 16 - (left & 15);
+        for (int i = lane; i < wide * rows * 8; i += 32) {
+          const int b = i / (rows * 8), r = left + (i >> 3) % rows;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(src + b * 8192 + r * 128 + (i & 7) * 16), "r"(0) : "memory");
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
         if (lane == 0) {
-          uint64_t da = operand<kALines>(src), db = operand<kBLines>(src + kABytes);
-          const int steps = min(kDepth / 16, (left + 15) / 16);
-          for (int i = 0; i < steps; ++i) {
-            mma(d, da, db, instr, k > 0 || i > 0);
-            da += operand_step<kALines>(), db += operand_step<kBLines>();
-          }
-          mma_commit(empty(s));
+          if (PAIR) mbar_arrive_remote(cleared(s), 0); else mbar_arrive(cleared(s));
         }
         __syncwarp();
-        if (++s == STAGES) s = 0, phase ^= 1;
       }
-      if (!ok) break;
-      if (lane == 0) {
-        if (t.stages)
-          mma_commit(acc_full(acc));
-        else
-          mbar_arrive(acc_full(acc));
-      }
-      __syncwarp();
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
+      s = (s + 1) % STAGES;
     }
   } else if (!TMA && warp >= kThreads / 32) {   // copies, line by line
     const int w = (warp - kThreads / 32) % kLoaders, team = (warp - kThreads / 32) / kLoaders;
@@ -460,7 +557,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     uint32_t phase = 0;
     bool ok = true;
     for (int u = first; u < units && ok; u += step) {
-      const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
+      const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
       for (int k = 0; k < t.stages; ++k) {
         const int at = s;
         const uint32_t parity = phase ^ 1;
@@ -490,10 +587,13 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     }
   } else if (warp >= 4) {   // results
     const int q = warp - 4;
+    auto acc_left = [&](int b) {   // whoever issues the products may write it again
+      if (PAIR) mbar_arrive_remote(acc_empty(b), 0); else mbar_arrive(acc_empty(b));
+    };
     int acc = 0;
     uint32_t acc_phase = 0, part_phase = 0;
     for (int u = first; u < units; u += step) {
-      const tile t = tile_at<MODE, BN, CL>(a, ends, slot_ends, u, rank);
+      const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
       if (!mbar_wait(acc_full(acc), acc_phase, &failed)) break;
       tensor_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(q * 32) << 16);
@@ -513,7 +613,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         }
         tensor_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty(acc));
+        if (lane == 0) acc_left(acc);
       } else if (CL == 1) {
         for (int c = 0; c < t.rows; c += 32) {
           uint32_t v[32];
@@ -530,7 +630,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         }
         tensor_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty(acc));
+        if (lane == 0) acc_left(acc);
       } else {
         // Every block takes 1 / CL of the tile's rows and gets the others' parts of them pushed into its shared memory.
         const int share = (t.rows + 15) / 16 * 16 / CL;
@@ -571,7 +671,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
-  } else if (!kWeight && a.zero_rows) {   // rows of no group, by the two warps that are left
+  } else if (!kWeight && a.zero_rows && (warp == 2 || warp == 3)) {   // rows of no group, by the two warps that are left
     typedef typename raw_bytes<TMA ? 16 : 2>::type word;
     const int64_t width = TMA ? a.cols / 8 : a.cols;     // words to a row
     word* words = reinterpret_cast<word*>(out);
@@ -589,13 +689,13 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     const long long begin = clock64();
     while (clock64() - begin < 4000000ll) __nanosleep(1000);
   }
-  if (CL > 1) {   // nobody pushes into the memory of a block that has left
+  if (kBlocks > 1) {   // nobody reaches into the memory of a block that has left
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   if (warp == 2) {
     tensor_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kColumns) : "memory");
+    tensor_free<PAIR, kColumns>(tmem);
   }
 }
 
@@ -621,11 +721,11 @@ bool encode(CUtensorMap* map, bool half, const void* p, int dims, const int64_t*
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int MODE, int BN, int STAGES, int CL, bool TMA>
+template <typename T, int MODE, int BN, int STAGES, int CL, bool TMA, bool PAIR = false>
 cudaError_t launch_one(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* out, int64_t units,
                        cudaStream_t s) {
-  auto* kernel = grouped_tensor_kernel<T, MODE, BN, STAGES, CL, TMA>;
-  constexpr int smem = smem_bytes<BN, STAGES, CL>();
+  auto* kernel = grouped_tensor_kernel<T, MODE, BN, STAGES, CL, TMA, PAIR>;
+  constexpr int smem = smem_bytes<BN, STAGES, CL, PAIR>();
   // per call: the attribute belongs to the current device's context, and a process may drive several GPUs
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
@@ -633,11 +733,12 @@ cudaError_t launch_one(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap&
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = CL, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  constexpr int kBlocks = PAIR ? 2 : CL;
+  attr[1].val.clusterDim.x = kBlocks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3((unsigned)(std::min<int64_t>(units, ctx->sm_count / CL) * CL));
+  c.gridDim = dim3((unsigned)(std::min<int64_t>(units, ctx->sm_count / kBlocks) * kBlocks));
   c.blockDim = dim3(TMA ? kThreads : kThreads + kTeams * kLoaders * 32);
-  c.dynamicSmemBytes = smem, c.stream = s, c.attrs = attr, c.numAttrs = CL > 1 ? 2 : 1;
+  c.dynamicSmemBytes = smem, c.stream = s, c.attrs = attr, c.numAttrs = kBlocks > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&c, kernel, a, ma, mb, (T*)out);
   ctx->launches++;
   return e != cudaSuccess ? e : cudaGetLastError();
@@ -652,8 +753,14 @@ struct product_call {
   int64_t units;   // no more tiles than that
 };
 
+// Two blocks to a tile of 256 x 256: each fetches one half of either operand, 64 bytes for every 128 x 128 x 1 products where
+// a block alone fetches 96, more than the L2 cache delivers to all SMs at full speed.  Where the output is wide enough that its last
+// tile of 256 columns is not often half empty.
+bool pays_as_pair(int64_t cols) { return cols > kLanes && (cols >= 1024 || (cols - 1) % 256 >= 128); }
+
 template <typename T, int MODE, bool TMA>
 cudaError_t launch_product(hpspmm_ctx* ctx, const product_call& c, cudaStream_t s) {
+  if (TMA && c.wide && pays_as_pair(c.a.cols)) return launch_one<T, MODE, 256, 6, 1, true, true>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
   if (c.wide) return launch_one<T, MODE, 256, 4, 1, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
   const int stages = (c.a.depth + kDepth - 1) / kDepth;
   int cl = 8;
@@ -673,6 +780,7 @@ cudaError_t launch_product(hpspmm_ctx* ctx, const product_call& c, bool out_firs
 template <typename T>
 cudaError_t launch_weight_grad(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* dW, bool tma,
                                bool wide, int64_t units, cudaStream_t s) {
+  if (tma && wide && pays_as_pair(a.cols)) return launch_one<T, MODE_WEIGHT, 256, 6, 1, true, true>(ctx, a, ma, mb, dW, units, s);
   if (tma)
     return wide ? launch_one<T, MODE_WEIGHT, 256, 4, 1, true>(ctx, a, ma, mb, dW, units, s)
                 : launch_one<T, MODE_WEIGHT, 64, 8, 1, true>(ctx, a, ma, mb, dW, units, s);
