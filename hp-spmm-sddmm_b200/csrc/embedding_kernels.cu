@@ -154,11 +154,13 @@ digit_place_kernel(int64_t T, int N, const void* ids, int wide, const int* keys_
     if (d < digits) {
       int at = sum - all + of_digit_before[d];
       for (int w = 0; w < warp; ++w) at += warp_sum[w];
-#pragma unroll 8
+      int n[kSortWarps];
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) n[w] = places[w * digits + d];
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
-        const int n = places[w * digits + d];
         places[w * digits + d] = at;
-        at += n;
+        at += n[w];
       }
     }
   }
@@ -310,79 +312,115 @@ sum_parts_kernel(int n, int N, int K, int64_t parts, int slabs, int length, cons
   if (!last_is_row) to_split(1);
 }
 
-// Rows that lie in several parts.  A block has 8 parts, one to a warp, and 128 columns: a row that began earlier and ends in
-// the part is the sum of the pieces before it and its own.  The warps share the pieces of rows that have many.
-constexpr int kJoinColumns = 128;
+template <int E>
+__device__ __forceinline__ void load_columns(const float* p, float (&v)[E]) {
+  if (E == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x, v[1 % E] = x.y, v[2 % E] = x.z, v[3 % E] = x.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = p[i];
+  }
+}
 
-template <typename T>
+// Rows that lie in several parts: a row that began earlier and ends in a part is the sum of the pieces before it and its own.
+// A block has 16 parts and 512 columns, every gridDim.x-th part, since those with such rows lie together; those that end one are shared out among its warps, but for rows
+// of many pieces, on which all of them work.  (With a block to 8 parts and 128 columns most of the time went into blocks
+// without work: 81 us for 262,144 positions of 262,144 x 2048.)
+constexpr int kJoinParts = 16;
+constexpr int kJoinColumns = 512;
+constexpr int kJoinMany = 32;
+
+template <typename T, int E>   // E: columns that one load takes, 4 where all rows of `split` are aligned for it
 __global__ void __launch_bounds__(kThreads)
 join_parts_kernel(int N, int K, int64_t parts, const int2* info, const float* split, float scale, T* __restrict__ dtable) {
-  constexpr int kWarps = kThreads / 32;
-  __shared__ int64_t first_of[kWarps];
-  __shared__ int row_of[kWarps];
-  __shared__ float sums[kWarps][kJoinColumns];
+  constexpr int kWarps = kThreads / 32, kStep = 32 * E, kSteps = kJoinColumns / kStep;
+  __shared__ int64_t first_of[kJoinParts];
+  __shared__ int row_of[kJoinParts];
+  __shared__ float sums[kWarps][kStep];
   chain_grid();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t part = (int64_t)blockIdx.x * kWarps + warp;
-  const int col = blockIdx.y * kJoinColumns + lane;
-  int row = -1;
-  int64_t first = 0;
-  if (part < parts) {
-    const int2 here = info[part];
-    const int next = part + 1 < parts ? info[part + 1].x : N;
-    if (here.y && here.x < N && next > here.x) {
-      row = here.x;
-      int64_t lo = 0, n = part;   // first part that begins inside this row or at its first position: in [lo, lo + n]
-      while (n > 0) {
-        const int64_t step = n / 33 + 1, at = lo + (lane + 1) * step - 1;
-        const bool before = at < lo + n && info[at].x < row;
-        const int c = __popc(__ballot_sync(0xffffffffu, before));
-        lo += c * step;
-        n = min(n - c * step, step - 1);
-      }
-      first = info[lo].y ? lo - 1 : lo;   // (open: its beginning is the part in front)
+  auto part_of = [&](int i) { return (int64_t)i * gridDim.x + blockIdx.x; };
+  {   // two parts to a warp
+    const int i = warp * 2 + (lane >> 4), sub = lane & 15;
+    const unsigned mask = 0xffffu << (lane & 16);
+    const int64_t part = part_of(i);
+    int row = -1;
+    if (part < parts) {
+      const int2 here = info[part];
+      const int next = part + 1 < parts ? info[part + 1].x : N;
+      if (here.y && here.x < N && next > here.x) row = here.x;
+    }
+    int64_t lo = 0, n = row >= 0 ? part : 0;   // first part that begins inside this row or at its first position: in [lo, lo + n]
+    while (n > 0) {
+      const int64_t step = n / 17 + 1, at = lo + (sub + 1) * step - 1;
+      const bool before = at < lo + n && info[at].x < row;
+      const int c = __popc(__ballot_sync(mask, before) & mask);
+      lo += c * step;
+      n = min(n - c * step, step - 1);
+    }
+    if (sub == 0) {
+      row_of[i] = row;
+      first_of[i] = row >= 0 && info[lo].y ? lo - 1 : lo;   // (open: its beginning is the part in front)
     }
   }
-  // columns lane, lane + 32, ... of pieces [b, e)
-  auto add = [&](int64_t b, int64_t e, float (&sum)[4]) {
+  __syncthreads();
+  // pieces [b, e) in the E columns from `col` on
+  auto add = [&](int64_t b, int64_t e, int col, float (&sum)[E]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = 0.f;
-#pragma unroll 4
+    for (int i = 0; i < E; ++i) sum[i] = 0.f;
+    if (col >= K) return;
+    const float* p = split + (2 * b + 1) * K + col;
+#pragma unroll 8
     for (int64_t s = b; s < e; ++s) {
-      const float* p = split + (2 * s + 1) * K + col;
+      float v[E];
+      load_columns<E>(p, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col + 32 * i < K) sum[i] += p[32 * i];
+      for (int i = 0; i < E; ++i) sum[i] += v[i];
+      p += 2 * (int64_t)K;
     }
   };
-  const bool many = row >= 0 && part - first > 4 * kWarps;
-  if (row >= 0 && !many) {
-    float sum[4];
-    add(first, part, sum);
+  auto load_own = [&](int i, int col, float (&own)[E]) {
+    if (col < K) load_columns<E>(split + 2 * part_of(i) * K + col, own);
+  };
+  auto finish = [&](int i, int col, const float (&sum)[E], const float (&own)[E]) {
+    if (col >= K) return;
+    T* to = dtable + (int64_t)row_of[i] * K + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + 32 * i < K)
-        dtable[(int64_t)row * K + col + 32 * i] = from_float<T>(scale * (sum[i] + split[2 * part * K + col + 32 * i]));
-  }
-  if (lane == 0) row_of[warp] = many ? row : -1, first_of[warp] = first;
-  __syncthreads();
-  for (int w = 0; w < kWarps; ++w) {
-    const int r = row_of[w];
-    if (r < 0) continue;
-    const int64_t f = first_of[w], own = (int64_t)blockIdx.x * kWarps + w, pieces = own - f;
-    float sum[4];
-    add(f + pieces * warp / kWarps, f + pieces * (warp + 1) / kWarps, sum);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sums[warp][lane + 32 * i] = sum[i];
-    __syncthreads();
-    const int c = blockIdx.y * kJoinColumns + threadIdx.x;
-    if (threadIdx.x < kJoinColumns && c < K) {
-      float all = sums[0][threadIdx.x];
-#pragma unroll
-      for (int i = 1; i < kWarps; ++i) all += sums[i][threadIdx.x];
-      dtable[(int64_t)r * K + c] = from_float<T>(scale * (all + split[2 * own * K + c]));
+    for (int e = 0; e < E; ++e) to[e] = from_float<T>(scale * (sum[e] + own[e]));
+  };
+  const int col0 = blockIdx.y * kJoinColumns + lane * E;
+  const int steps = min(kSteps, (K - (int)blockIdx.y * kJoinColumns + kStep - 1) / kStep);
+  int turn = 0;
+  for (int i = 0; i < kJoinParts; ++i) {
+    if (row_of[i] < 0 || part_of(i) - first_of[i] > kJoinMany) continue;
+    for (int c = 0; c < steps; ++c) {
+      if (turn++ % kWarps != warp) continue;
+      float sum[E], own[E];
+      load_own(i, col0 + c * kStep, own);
+      add(first_of[i], part_of(i), col0 + c * kStep, sum);
+      finish(i, col0 + c * kStep, sum, own);
     }
-    __syncthreads();
+  }
+  for (int i = 0; i < kJoinParts; ++i) {
+    const int64_t f = first_of[i], pieces = part_of(i) - f;
+    if (row_of[i] < 0 || pieces <= kJoinMany) continue;
+    for (int c = 0; c < steps; ++c) {
+      float sum[E], own[E];
+      load_own(i, col0 + c * kStep, own);
+      add(f + pieces * warp / kWarps, f + pieces * (warp + 1) / kWarps, col0 + c * kStep, sum);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = sum[e];
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w)
+#pragma unroll
+          for (int e = 0; e < E; ++e) sum[e] += sums[w][lane * E + e];
+        finish(i, col0 + c * kStep, sum, own);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -398,7 +436,9 @@ struct backward_plan {
   size_t keys, pos, tables, info, split, bytes;   // offsets
 };
 
-// Places to a part: 64 amortise the search (4 rounds of 32 probes), 16 where there would be less than about a wave.
+// Places to a part: 16 to 256, as many as leave 48 warps for every SM (a slab of columns is 256 wide at least).  Longer
+// parts mean fewer rows in several of them: 64 instead of 256 cost 53 us instead of 17 in the join for 262,144 positions of
+// 262,144 x 2048.
 backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
   backward_plan p = {};
   while (p.bits < 31 && ((int64_t)1 << p.bits) <= N) ++p.bits;
@@ -410,7 +450,7 @@ backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
   if (T > 1 << 20) p.chunk = (T + 147) / 148;
   p.chunk = std::max<int64_t>(1, (p.chunk + kSortThreads - 1) / kSortThreads) * kSortThreads;
   p.blocks = (int)((T + p.chunk - 1) / p.chunk);
-  p.length = (T + N) * ((K + 255) / 256) < 148 * 32 * 64 ? 16 : 64;
+  p.length = (int)std::min<int64_t>(256, std::max<int64_t>(16, ((T + N) * ((K + 255) / 256) / (148 * 48) + 15) / 16 * 16));
   p.parts = (T + N + p.length - 1) / p.length;
   const size_t b_t = align_up((size_t)T * 4, 256);
   p.keys = 0;
@@ -460,8 +500,13 @@ void launch_sums(hpspmm_ctx* ctx, const backward_plan& p, int64_t n, int64_t N, 
   hpspmm_launch(sum_parts_kernel<T, BYTES, R, W>, dim3((unsigned)((lanes + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, (int)n, (int)N,
                 (int)K, p.parts, (int)slabs, p.length, keys, pos, (const T*)dout, ld, scale, (T*)dtable, (int2*)(space + p.info),
                 (float*)(space + p.split));
-  hpspmm_launch(join_parts_kernel<T>, dim3((unsigned)((p.parts + kThreads / 32 - 1) / (kThreads / 32)), (unsigned)((K + kJoinColumns - 1) / kJoinColumns)),
-                dim3(kThreads), 0, s, (int)N, (int)K, p.parts, (const int2*)(space + p.info), (const float*)(space + p.split), scale, (T*)dtable);
+  const dim3 grid((unsigned)((p.parts + kJoinParts - 1) / kJoinParts), (unsigned)((K + kJoinColumns - 1) / kJoinColumns));
+  const int2* info = (const int2*)(space + p.info);
+  const float* split = (const float*)(space + p.split);
+  if (K % 4 == 0)
+    hpspmm_launch(join_parts_kernel<T, 4>, grid, dim3(kThreads), 0, s, (int)N, (int)K, p.parts, info, split, scale, (T*)dtable);
+  else
+    hpspmm_launch(join_parts_kernel<T, 1>, grid, dim3(kThreads), 0, s, (int)N, (int)K, p.parts, info, split, scale, (T*)dtable);
   ctx->launches += 2;
 }
 
@@ -573,7 +618,7 @@ int hpspmm_embedding_backward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, 
   HPSPMM_REQUIRE(ctx, T == 0 || workspace_bytes >= p.bytes, "workspace too small");
   HPSPMM_REQUIRE(ctx, T == 0 || ((uintptr_t)workspace & 255) == 0, "workspace not aligned to 256 bytes");
   if (p.parts * ((K + 31) / 32) > (int64_t)2147483647 * 8 || K > (int64_t)65535 * kJoinColumns)
-    return hpspmm_unsupported(ctx, "more than 2^31 - 1 blocks, or 8,388,480 columns");
+    return hpspmm_unsupported(ctx, "more than 2^31 - 1 blocks, or 33,553,920 columns");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   if (T == 0) {

@@ -66,15 +66,20 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar, int rank) {
       "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
       " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(bar), "r"(rank) : "memory");
 }
+// A wait may sleep that many nanoseconds in the hardware.  Without the hint six of the eight warps polled, which on a GPU at
+// its power limit was taken from the products: 1979 us for what takes 1859 (32,768 rows of 8 groups, 2048 x 5632, with both
+// gradients, over 1.5 s).
+constexpr uint32_t kSleep = 1000000;
+
 template <bool CLUSTER>
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   if (CLUSTER)
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(kSleep) : "memory");
   else
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(kSleep) : "memory");
   return ok != 0;
 }
 // Waits for at most about two seconds.  Whoever gives up says so in `failed`, and all others give up with it.
@@ -461,9 +466,12 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     __syncwarp();
   } else if (warp == 1) {
     // Products, by one thread (of a pair: the first block's).  The next instruction has to be there when the one before it
-    // ends, 128 cycles later: with the whole warp on its way through the loop and the next tile looked up between two of them
-    // the tensor cores stood still for a third of the time.
-    if (lane == 0 && !(PAIR && rank)) {
+    // ends, 128 cycles later.  With the next tile looked up between two tiles the tensor cores stood still for a third of the
+    // time; a look at the next stage's barrier between two products of one cost 10 %; and the warp stays together, so that
+    // descriptors are kept in uniform registers: 3 % ahead of one lane on its own.
+    if (!(PAIR && rank)) {
+      uint32_t one;
+      asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
       struct {
         int stages, rows, steps;   // steps: of 16 of the depth, in the last stage
         bool cut;
@@ -474,6 +482,9 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         const int left = (kWeight ? t.end - t.begin : a.depth - t.begin * kDepth) - (t.stages - 1) * kDepth;
         next.stages = t.stages, next.rows = t.rows, next.steps = min(kDepth / 16, (left + 15) / 16);
         next.cut = kWeight && TMA && t.stages > 0 && cut_short(t, t.stages - 1);
+        // (the same in all lanes, and known to be)
+        next.stages = __shfl_sync(0xffffffffu, next.stages, 0), next.rows = __shfl_sync(0xffffffffu, next.rows, 0);
+        next.steps = __shfl_sync(0xffffffffu, next.steps, 0), next.cut = __shfl_sync(0xffffffffu, (int)next.cut, 0);
       };
       const uint64_t first_a = operand<kALines>(base), first_b = operand<kBLines>(base + kABytes);
       int s = 0, acc = 0;
@@ -503,22 +514,28 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
           tensor_fence_after();
           const uint64_t da = first_a + (uint64_t)(s * (kStage >> 4)), db = first_b + (uint64_t)(s * (kStage >> 4));
           const int steps = last ? w.steps : kDepth / 16;
-          mma<PAIR>(d, da, db, instr, k > 0);
+          if (one) {
+            mma<PAIR>(d, da, db, instr, k > 0);
 #pragma unroll
-          for (int i = 1; i < kDepth / 16; ++i)
-            if (i < steps) mma<PAIR>(d, da + i * operand_step<kALines>(), db + i * operand_step<kBLines>(), instr, true);
-          mma_commit<PAIR>(empty(s));
+            for (int i = 1; i < kDepth / 16; ++i)
+              if (i < steps) mma<PAIR>(d, da + i * operand_step<kALines>(), db + i * operand_step<kBLines>(), instr, true);
+            mma_commit<PAIR>(empty(s));
+          }
+          __syncwarp();
           if (k == 0) look_up(u + step);
           if (++s == STAGES) s = 0;
         }
         if (!ok) break;
-        if (w.stages) {
-          mma_commit<PAIR>(acc_full(acc));
-        } else {
-          look_up(u + step);
-          mbar_arrive(acc_full(acc));
-          if (PAIR) mbar_arrive_remote(acc_full(acc), 1);
+        if (w.stages == 0) look_up(u + step);
+        if (one) {
+          if (w.stages) {
+            mma_commit<PAIR>(acc_full(acc));
+          } else {
+            mbar_arrive(acc_full(acc));
+            if (PAIR) mbar_arrive_remote(acc_full(acc), 1);
+          }
         }
+        __syncwarp();
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
