@@ -393,6 +393,14 @@ TORCH_LIBRARY_IMPL(hpspmm, Autograd, m) {
 
 // The operators without the Python dispatcher's share.
 void bind_dense_operators(py::module_& m) {
+  m.def("timeouts", [](int device) {
+    DeviceContext& c = context_of(at::Device(at::kCUDA, (c10::DeviceIndex)device));
+    int64_t n = 0;
+    std::lock_guard<std::mutex> lock(c.use);
+    const int st = hpspmm_ctx_timeouts(c.ctx, &n);
+    TORCH_CHECK(st == HPSPMM_OK, "hpspmm_ctx_timeouts failed with status ", st, ": ", hpspmm_last_error(c.ctx));
+    return n;
+  }, py::call_guard<py::gil_scoped_release>());
   m.def("embedding", [](const Tensor& ids, const Tensor& table, double scale) { return op_embedding().call(ids, table, scale); },
         py::call_guard<py::gil_scoped_release>());
   m.def("grouped_product",

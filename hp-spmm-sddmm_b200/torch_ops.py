@@ -187,3 +187,10 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0):
     if _plain(logits, teacher_ids, teacher_logits):
         return _C.topk_distill(logits, teacher_ids, teacher_logits, temperature)
     return torch.ops.hpspmm.topk_distill.default(logits, teacher_ids, teacher_logits, temperature)[0]
+
+
+def timeouts(device=None):
+    """How many blocks of the grouped products' tensor-core kernels have given up a wait on this GPU (expected 0; what
+    such a call wrote is not to be used).  Waits for the device."""
+    index = None if device is None else torch.device(device).index
+    return _C.timeouts(torch.cuda.current_device() if index is None else index)

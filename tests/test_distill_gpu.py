@@ -290,3 +290,73 @@ def test_the_operators_pass_through_a_tracer(ops):
             fake = op(*[mode.from_tensor(a) if isinstance(a, torch.Tensor) else a for a in args])
         for r, f in zip(real if isinstance(real, tuple) else (real,), fake if isinstance(fake, tuple) else (fake,)):
             assert (r.shape, r.dtype, r.stride()) == (f.shape, f.dtype, f.stride())
+
+
+def test_a_captured_training_step(ops):
+    """Lookup, product by group and loss with all their gradients as one graph, replayed on new inputs."""
+    gen = torch.Generator("cuda").manual_seed(12)
+    T, rows, K, V = 3000, 700, 64, 520
+    ids, offsets = torch.zeros(T, dtype=torch.int64, device="cuda"), torch.tensor([0, 1000, 1010, 3000], dtype=torch.int32, device="cuda")
+    top, teacher = torch.zeros((T, 8), dtype=torch.int64, device="cuda"), torch.zeros((T, 8), device="cuda")
+    table = torch.randn((rows, K), device="cuda", generator=gen).bfloat16().requires_grad_()
+    W = (torch.randn((3, K, V), device="cuda", generator=gen) / 8).bfloat16().requires_grad_()
+
+    def step():
+        z = ops.grouped_product(ops.embedding(ids, table, 2.0), W, offsets)
+        loss = ops.topk_distill_loss(z, top, teacher, 2.0).mean()
+        return (loss.detach(), *torch.autograd.grad(loss, (table, W)))
+
+    def fill():
+        ids.copy_(torch.randint(-1, rows, (T,), device="cuda", generator=gen))
+        top.copy_(torch.randint(-1, V, (T, 8), device="cuda", generator=gen))
+        teacher.copy_(torch.randn((T, 8), device="cuda", generator=gen))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fill()
+        step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        held = step()
+    for _ in range(3):
+        fill()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager))
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Contexts and kernels are made ready there and then."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+import __graft_entry__
+import dense_reference as ref
+ops = ref.ops_of(__graft_entry__.load_package())
+ids, table = torch.tensor([1, 0, -1], device="cuda"), torch.randn((2, 64), device="cuda").bfloat16()
+W, off = torch.randn((2, 64, 32), device="cuda").bfloat16(), torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+top, teacher = torch.tensor([[3], [4], [5]], device="cuda"), torch.zeros((3, 1), device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    x = ops.embedding(ids, table)
+    z = ops.grouped_product(x, W, off)
+    loss = ops.topk_distill_loss(z, top, teacher)
+g.replay()
+torch.cuda.synchronize()
+want, tol = ref.grouped(x, W, off)
+assert ref.outside(z, want, tol) == 0 and torch.equal(x[0], table[1]) and not x[2].any()
+want, tol = ref.distill(z, top, teacher, 1.0)
+assert ref.outside(loss, want, tol) == 0
+print("well")
+""" % (root, os.path.join(root, "tests"))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip().endswith("well"), out.stdout[-2000:]

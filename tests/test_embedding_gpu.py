@@ -221,3 +221,19 @@ def test_refusals(ops, pkg, gpu_ctx):
         with pytest.raises(pkg.HpspmmError):
             gpu_ctx.embedding_backward(*(good[:at] + [v] + good[at + 1:]))
     assert pkg.load_library().hpspmm_embedding_backward_workspace(-1, 4, 8) == -1
+    with pytest.raises(pkg.HpspmmError):
+        gpu_ctx.embedding_backward(*(good[:10] + [space.data_ptr() + 8, need]))
+
+
+def test_one_row_of_the_gradient_for_all_positions(pkg, gpu_ctx):
+    """A row stride of zero, as of a sum over the positions: read as it lies."""
+    ids = torch.tensor([2, 0, 2, 5, -1, 2], dtype=torch.int32, device="cuda")
+    row, dtable = torch.randn(40, device="cuda"), torch.full((4, 40), 7.0, device="cuda")
+    need = pkg.load_library().hpspmm_embedding_backward_workspace(6, 4, 40)
+    space = torch.empty(need, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.embedding_backward(6, 4, 40, pkg.TYPE_F32, ids.data_ptr(), 4, row.data_ptr(), 0, 1.0, dtable.data_ptr(),
+                               space.data_ptr(), need)
+    torch.cuda.synchronize()
+    assert torch.equal(dtable[0], row) and not dtable[1].any() and not dtable[3].any()
+    assert float((dtable[2].double() - 3 * row.double()).abs().max()) <= 3 * 2.0 ** -23 * float(row.abs().max())

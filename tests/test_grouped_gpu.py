@@ -300,3 +300,69 @@ def test_groups_cut_into_pieces(ops, type, sizes, K, N):
     n = sum(sizes)
     off = torch.tensor([0, n] * 3 + [0], dtype=torch.int32, device="cuda")
     assert torch.ops.hpspmm.grouped_weight_grad(X, dY, off, False).shape == (6, K, N)
+
+
+# enough tiles for blocks of 256 rows: pairs of blocks (1024 columns), blocks by themselves (384), rows that no copy engine
+# takes (odd widths)
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("sizes,K,N", [([4000, 0, 3000, 33], 256, 1024), ([300] * 40 + [1, 15, 17], 1024, 2048), ([6000, 0, 7001, 500], 72, 384),
+                                       ([1500, 1, 4000, 0, 777], 70, 1031), ([511, 513, 3, 2048, 70, 900], 1024, 1100)])
+def test_many_tiles(ops, type, sizes, K, N):
+    gen = torch.Generator("cuda").manual_seed(N)
+    R = sum(sizes) + 40
+    X, dY = (torch.randn((R, c), device="cuda", generator=gen).to(ref.TYPES[type]) for c in (K, N))
+    X[sum(sizes):], dY[sum(sizes):] = float("nan"), float("inf")        # rows behind the last group
+    for transposed in (False, True):
+        W = _weights(len(sizes), K, N, X.dtype, gen, transposed)
+        y, dx, dw = _check(ops, X, W, _offsets(sizes), dY)
+        assert not y[sum(sizes):].any() and not dx[sum(sizes):].any()
+        again = _check(ops, X, W, _offsets(sizes), dY)
+        assert all(torch.equal(a, b) for a, b in zip((y, dx, dw), again))
+
+
+def test_neighbours_of_a_group_do_not_reach_its_gradient(ops):
+    """Groups that end inside the 16 rows of an instruction, between groups of NaN: pairs of blocks and single ones."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    for K, N in ((1024, 2048), (72, 384), (64, 64)):
+        sizes = [37, 64, 30, 1, 50, 5, 100] * 6
+        off = _offsets(sizes)
+        X, dY = (torch.randn((sum(sizes), c), device="cuda", generator=gen).bfloat16() for c in (K, N))
+        want, tol = ref.grouped_weight(X, dY, off)
+        bounds = off.tolist()
+        for g in range(1, len(sizes), 2):
+            X[bounds[g]:bounds[g + 1]], dY[bounds[g]:bounds[g + 1]] = float("nan"), float("inf")
+        for transposed in (False, True):
+            dw = torch.ops.hpspmm.grouped_weight_grad(X, dY, off, transposed)
+            assert ref.outside(dw[::2], want[::2], tol[::2]) == 0 and bool(torch.isnan(dw[1::2]).all())
+
+
+def test_streams_and_threads_at_once(ops):
+    """Calls of several threads, each on a stream of its own, without waiting for one another."""
+    import threading
+    gen = torch.Generator("cuda").manual_seed(11)
+    work, errors = [], []
+    for i, (K, N, dtype) in enumerate(((1024, 1024, torch.bfloat16), (50, 30, torch.float32), (2048, 128, torch.float16))):
+        sizes = [30 * (i + 1), 0, 700]
+        X = torch.randn((sum(sizes), K), device="cuda", generator=gen).to(dtype)
+        dY = torch.randn((sum(sizes), N), device="cuda", generator=gen).to(dtype)
+        W = _weights(3, K, N, dtype, gen, False)
+        work.append((X, dY, W, _offsets(sizes), ref.grouped(X, W, _offsets(sizes)), ref.grouped_weight(X, dY, _offsets(sizes))))
+    torch.cuda.synchronize()
+
+    def steps(X, dY, W, off, want, want_w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(40):
+                    y, dw = ops.grouped_product(X, W, off), torch.ops.hpspmm.grouped_weight_grad(X, dY, off, False)
+                    if i % 10 == 9:
+                        assert ref.outside(y, *want) == 0 and ref.outside(dw, *want_w) == 0
+        except BaseException as e:      # noqa: B902 -- a thread's failure is the test's
+            errors.append(e)
+
+    threads = [threading.Thread(target=steps, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
+    assert ops.timeouts() == 0
