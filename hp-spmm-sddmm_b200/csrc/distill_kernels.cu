@@ -17,7 +17,10 @@ using namespace hpspmm;
 constexpr int kThreads = 256;
 constexpr int kMaxEntries = 1024;   // of the teacher for one row
 constexpr int kMaxEntriesWarp = 64; // where a warp has a row
-constexpr int kVectors = 4;         // of 16 bytes in flight per thread
+// Vectors of 16 bytes in flight per thread.  4,096 x 131,072 bf16: backward 357 us with four, 346 with eight; forward with
+// four 185 us where six blocks to an SM are asked for, 196 without (1,021 x 32,003 floats: 39 and 32).
+constexpr int kForwardVectors = 4;
+constexpr int kBackwardVectors = 8;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // (within 2^-22 of the value; results below 2^-126 are zero)
@@ -100,11 +103,11 @@ struct running {
 // One pass over the row, everything in registers: NT threads to a row, CL blocks of a cluster to one where rows are few.
 // Bound by the reads of the logits; an element costs one ex2 and about five other instructions.
 template <typename T, int NT, int CL>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 0)
 distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
                        const float* __restrict__ teacher, float tau, float* __restrict__ loss, float2* __restrict__ stats) {
   typedef dense_vec<T, 16> vec;
-  constexpr int E = vec::kCount;
+  constexpr int E = vec::kCount, kTogether = 8 / E;   // eight values to a step
   constexpr int kRows = kThreads / NT, kEntries = NT == 32 ? kMaxEntriesWarp : kMaxEntries;
   __shared__ float of_teacher[kRows][kEntries], of_student[kRows][kEntries];   // logits at the teacher's entries
   __shared__ float part[kThreads / 32];
@@ -130,15 +133,15 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
   const uint4* words = reinterpret_cast<const uint4*>(z + at.head);
   const int begin = (int)((int64_t)at.vectors * rank / CL), end = (int)((int64_t)at.vectors * (rank + 1) / CL);
   int v = begin + tid;
-  for (; v + (kVectors - 1) * NT < end; v += kVectors * NT) {
-    vec x[kVectors];
+  for (; v + (kForwardVectors - 1) * NT < end; v += kForwardVectors * NT) {
+    vec x[kForwardVectors];
 #pragma unroll
-    for (int u = 0; u < kVectors; ++u) x[u].raw = __ldg(words + v + u * NT);
+    for (int u = 0; u < kForwardVectors; ++u) x[u].raw = __ldg(words + v + u * NT);
 #pragma unroll
-    for (int u = 0; u < kVectors; u += 2) {
-      float f[2 * E];
+    for (int u = 0; u < kForwardVectors; u += kTogether) {
+      float f[8];
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = to_float(x[u].at[e]), f[E + e] = to_float(x[u + 1].at[e]);
+      for (int e = 0; e < 8; ++e) f[e] = to_float(x[u + e / E].at[e % E]);
       r.add(f, c);
     }
   }
@@ -252,13 +255,13 @@ distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits
   }
   const uint4* words = reinterpret_cast<const uint4*>(z + at.head);
   uint4* out = reinterpret_cast<uint4*>(dz + at.head);
-  for (int v0 = begin + tid; v0 < end; v0 += kVectors * NT) {
-    vec x[kVectors];
+  for (int v0 = begin + tid; v0 < end; v0 += kBackwardVectors * NT) {
+    vec x[kBackwardVectors];
 #pragma unroll
-    for (int u = 0; u < kVectors; ++u)
+    for (int u = 0; u < kBackwardVectors; ++u)
       if (v0 + u * NT < end) x[u].raw = __ldg(words + v0 + u * NT);
 #pragma unroll
-    for (int u = 0; u < kVectors; ++u)
+    for (int u = 0; u < kBackwardVectors; ++u)
       if (v0 + u * NT < end) {
 #pragma unroll
         for (int e = 0; e < E; ++e) x[u].at[e] = from_float<T>(value(to_float(x[u].at[e])));
@@ -284,15 +287,17 @@ distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits
   }
 }
 
-// A warp to a row where rows are short and many enough to fill the warps; blocks to a row where there are few rows, each with
-// at least 16 KB of it.
+// A warp to a row where rows are short; several blocks, each with at least 32 KB of it, to a row where the rows do not fill
+// the SMs twice.  (Two or four to a row for more rows than that lost: 1,021 rows of 32,003 floats 32 us with one, 44 with
+// four: what a row costs beside its reads comes with every block.)
 struct distill_shape {
   bool warp;
   int parts;
 };
 distill_shape choose_distill(const hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int size) {
   distill_shape sh = {V * size <= 4096 && k <= kMaxEntriesWarp, 1};
-  while (!sh.warp && sh.parts < 8 && T * sh.parts < 2 * ctx->sm_count && V * size >= (int64_t)sh.parts * 32768) sh.parts *= 2;
+  while (!sh.warp && sh.parts < 8 && T * sh.parts < 2 * ctx->sm_count && V * size >= (int64_t)sh.parts * 32768)
+    sh.parts *= 2;
   return sh;
 }
 
