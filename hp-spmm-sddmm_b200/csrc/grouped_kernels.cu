@@ -3,6 +3,7 @@
 //   dW[g] = X_g^T * dY_g      over the rows of group g;  a group without rows gets zeros
 // (dX is the first one again, with dY and the matrices the other way round.)
 #include <algorithm>
+#include <cmath>
 
 #include "dense_types.cuh"
 #include "device_utils.cuh"
@@ -343,17 +344,28 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // Columns of a tile: 64 where that covers the output, as a matrix of a relation type often is that narrow.
 int64_t tile_columns(int64_t cols) { return cols <= 64 ? 64 : 128; }
 
-// Rows to a piece.  Ordinary cores: enough pieces for four blocks on each SM, if they have 256 rows (a tile takes about 10 us
-// for them); tensor cores: for two rounds of the SMs, if they have 1024 rows (about 4 us, against 2 to 3 for the 128 KB of a
-// tile in 32 bits).  All the rows where there are tiles enough.
+// Rows to a piece: all of them, or as many as fill the GPU once where that is expected to be faster.  In us: what 64 rows
+// take a tile (0.30 to 0.47 on the tensor cores, less with fewer tiles, which are smaller then, 1.65 without TMA; 9.6 or, 64 columns wide, 4.8
+// on the ordinary ones, which run two of them on an SM); whole groups take as long as the largest one, for which twice the
+// mean is assumed; pieces have at least 1024 (256) rows, take another launch and the way of their sums to memory and back
+// (4 TB/s; somewhat more than half of the slots are used).  16 groups of 750 rows, 1024 x 1024: 73 us in pieces, 31 whole; one group of 12,000, 4096 x 512: 59 us in pieces,
+// 71 whole; in 32 bits 16 groups of 750 rows, 512 x 512: 175 us in pieces, 270 whole.
 piece_plan plan_pieces(int64_t R, int64_t G, int64_t I, int64_t J, int32_t type) {
   const bool f32 = type == HPSPMM_TYPE_F32;
-  const int64_t bi = f32 ? kGradientRows : 256, bj = f32 ? tile_columns(J) : 128;
-  const int64_t tiles = ((I + bi - 1) / bi) * ((J + bj - 1) / bj), target = 148 * (f32 ? 4 : 2);
-  int64_t length = R;
-  if (tiles < target && G <= kMostSplitGroups) length = std::max<int64_t>(f32 ? 256 : 1024, (R * tiles / target + 63) / 64 * 64);
-  length = std::max<int64_t>(1, std::min(length, R));
-  return {(int)length, (int)piece_slots(R, length)};
+  const int64_t bi = f32 ? kGradientRows : 256, bj = f32 ? tile_columns(J) : 128, least = f32 ? 256 : 1024;
+  const int64_t tiles = ((I + bi - 1) / bi) * ((J + bj - 1) / bj), at_once = f32 ? 296 : 148;
+  piece_plan whole = {(int)std::max<int64_t>(1, R), 0};
+  if (G > kMostSplitGroups || R <= least || tiles >= at_once) return whole;
+  const int64_t length = std::min(R, std::max(least, (R * tiles / at_once + 63) / 64 * 64));
+  const piece_plan p = {(int)length, (int)piece_slots(R, length)};
+  const bool lines = I % 8 != 0 || J % 8 != 0;   // rows that TMA does not take
+  const double us = f32 ? (bj == 64 ? 4.8 : 9.6) : (lines ? 1.65 : 0.47);
+  const double us_whole = f32 || lines || G * tiles >= 100 ? us : (G * tiles < 50 ? 0.3 : 0.4);
+  const double rows = (double)R, largest = G == 1 ? rows : std::min(rows, 2 * rows / (double)G);
+  const double t_whole = std::ceil((double)(G * tiles) / (double)at_once) * largest / 64 * us_whole;
+  const double t_pieces = rows * (double)tiles / 64 * us / (double)at_once + 0.6 * (double)length / 64 * us + 7 +
+                          0.6 * (double)p.slots * (double)I * (double)J * 8 / 4e6;
+  return t_pieces < t_whole ? p : whole;
 }
 
 int check_grouped(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type) {

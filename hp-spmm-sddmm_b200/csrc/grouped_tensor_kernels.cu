@@ -14,6 +14,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "dense_types.cuh"
 #include "device_utils.cuh"
@@ -119,6 +120,8 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, u
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
                  "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t in_block(uint32_t addr, int rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -271,10 +274,6 @@ struct type_code<__half> { static constexpr uint32_t value = 0; };
 template <>
 struct type_code<__nv_bfloat16> { static constexpr uint32_t value = 1; };
 
-// rows to a TMA box of the N-side operand: few where tiles are small, so that little is fetched for nothing
-template <int BN>
-__host__ __device__ constexpr int box_rows() { return BN >= 128 ? 64 : 16; }
-
 // ---- tiles without TMA ---------------------------------------------------------------------------------------------
 //
 // Operands whose rows do not begin on 16-byte boundaries: eight warps bring a tile in, two such teams in turn, 128 bytes of
@@ -335,7 +334,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   constexpr int kBlocks = PAIR ? 2 : CL;                                 // of a cluster
   static_assert(!PAIR || (CL == 1 && TMA), "pairs neither split the depth nor go without TMA");
   // of the N side, a block of a pair holds one half
-  constexpr int kBBytes = BN * 128 / (PAIR ? 2 : 1), kStage = kABytes + kBBytes, kBox = box_rows<BN>();
+  constexpr int kBBytes = BN * 128 / (PAIR ? 2 : 1), kStage = kABytes + kBBytes;
   constexpr int kColumns = 2 * BN < 32 ? 32 : 2 * BN;                   // of tensor memory: two accumulators
   extern __shared__ char raw[];
   __shared__ int ends[kMaxGroups];
@@ -415,10 +414,10 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   if (!kWeight || a.plan.slots) prefix(ends, false);
   if (kWeight && a.plan.slots) prefix(slot_ends, true);
   __syncthreads();
-  if (kBlocks > 1) {   // the others' barriers are ready
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
+  // The others' barriers are ready: a pair needs them from the first copy on, blocks that split the depth only when they join
+  // their parts, and whoever does not waits at the end.
+  if (kBlocks > 1) cluster_arrive();
+  if (PAIR) cluster_wait();
   tensor_fence_after();
   const uint32_t tmem = tmem_base;
   const int units = tile_count<MODE, BN, PAIR ? 2 * kLanes : kLanes>(a, ends);
@@ -434,7 +433,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         // of the N side, this block's part: rows [from, from + count)
         const int half = (t.rows + 31) / 32 * 16;
         const int from = t.row0 + (PAIR ? rank * half : 0), count = PAIR ? half : t.rows;
-        const int boxes = (count + kBox - 1) / kBox;
+        const int boxes = (count + 63) / 64;
         for (int k = 0; k < t.stages; ++k) {
           ok = mbar_wait(empty(s), phase ^ 1, &failed);
           if (!ok) break;
@@ -442,13 +441,13 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
           // its own, in either block: its rest has to be cleared before it is used.
           const bool cut = kWeight && cut_short(t, k), shared = PAIR && !cut;
           const uint32_t dst = base + s * kStage, own = cut ? cut_full(s) : full(s), bar = shared ? in_block(own, 0) : own;
-          const uint32_t bytes = kABytes + (kWeight ? (count + 63) / 64 * 8192 : boxes * kBox * 128);
+          const uint32_t bytes = kABytes + boxes * 8192;
           if (!shared || rank == 0) mbar_expect(own, shared ? 2 * bytes : bytes);
           if (kWeight) {
-            const int wide = (count + 63) / 64, r = t.begin + k * kDepth;
+            const int r = t.begin + k * kDepth;
             tma_load<PAIR>(dst, &map_a, bar, t.col0, r);
             tma_load<PAIR>(dst + 8192, &map_a, bar, t.col0 + 64, r);
-            for (int b = 0; b < wide; ++b) tma_load<PAIR>(dst + kABytes + b * 8192, &map_b, bar, from + b * 64, r);
+            for (int b = 0; b < boxes; ++b) tma_load<PAIR>(dst + kABytes + b * 8192, &map_b, bar, from + b * 64, r);
           } else {
             const int d = (t.begin + k) * kDepth;
             if (MODE == MODE_OUT_FIRST) {
@@ -457,7 +456,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
               tma_load<PAIR>(dst, &map_a, bar, t.col0, d, t.g);
               tma_load<PAIR>(dst + 8192, &map_a, bar, t.col0 + 64, d, t.g);
             }
-            for (int b = 0; b < boxes; ++b) tma_load<PAIR>(dst + kABytes + b * kBox * 128, &map_b, bar, d, from + b * kBox);
+            for (int b = 0; b < boxes; ++b) tma_load<PAIR>(dst + kABytes + b * 8192, &map_b, bar, d, from + b * 64);
           }
           if (++s == STAGES) s = 0, phase ^= 1;
         }
@@ -609,6 +608,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     };
     int acc = 0;
     uint32_t acc_phase = 0, part_phase = 0;
+    if (CL > 1) cluster_wait();
     for (int u = first; u < units; u += step) {
       const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
       if (!mbar_wait(acc_full(acc), acc_phase, &failed)) break;
@@ -652,16 +652,21 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         // Every block takes 1 / CL of the tile's rows and gets the others' parts of them pushed into its shared memory.
         const int share = (t.rows + 15) / 16 * 16 / CL;
         if (!mbar_wait<true>(parts_empty, part_phase ^ 1, &failed)) break;
+        const uint32_t mine = smem_of(parts + rank * share * kLanes + q * 32 + lane);
+        int to_rank = 0, r = 0;
+        uint32_t at = in_block(mine, 0);
         for (int c = 0; c < CL * share; c += 32) {
           uint32_t v[32];
           tensor_load(src + c, v);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             if (c + j < CL * share) {
-              const int to_rank = (c + j) / share, r = c + j - to_rank * share;
-              const uint32_t at = smem_of(parts + (rank * share + r) * kLanes + q * 32 + lane);
-              asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n st.shared::cluster.b32 [a], %2;\n}\n" ::"r"(at),
-                           "r"(to_rank), "r"(v[j]) : "memory");
+              asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(v[j]) : "memory");
+              at += kLanes * 4;
+              if (++r == share) {
+                r = 0, ++to_rank;
+                if (to_rank < CL) at = in_block(mine, to_rank);
+              }
             }
           }
         }
@@ -707,8 +712,10 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     while (clock64() - begin < 4000000ll) __nanosleep(1000);
   }
   if (kBlocks > 1) {   // nobody reaches into the memory of a block that has left
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (CL > 1 && (warp < 4 || warp >= kThreads / 32)) cluster_wait();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
   }
   if (warp == 2) {
     tensor_fence_after();
@@ -761,30 +768,84 @@ cudaError_t launch_one(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap&
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// Rows (of dW: rows of the output) to a tile, whether pairs of blocks take it, and how many blocks split its depth.
+struct tile_choice {
+  int rows;
+  bool pair;
+  int blocks;
+};
+
+// Two blocks to a tile of 256 x 256: each fetches one half of either operand, 64 bytes for every 128 x 128 x 1 products where
+// a block alone fetches 96.  Where the output is wide enough that its last tile of 256 columns is not often half empty.
+bool wide_enough_for_pairs(int64_t cols) { return cols > kLanes && (cols >= 1024 || (cols - 1) % 256 >= 128); }
+
+// The choice for a product, from what was measured for a block's tile of 64, 128 or 256 rows and a pair's of 256 (1,024 to
+// 5,632 wide, depth 64 to 4,096, 8 to 30,000 rows of 1 to 64 groups): `stage` us for 64 of the depth, `rest` for the tile,
+// and not less than `store`, its way to memory.  The host does not know the groups' sizes: half a tile more than the rows
+// need for each of them is assumed.  1,500 rows of one group, 2048 x 2048: 44 us with tiles of 64, 27 with 128, 19 with 256,
+// 18 with pairs; 600 rows 22 / 16 / 18 / 17; 30,000 rows, 64 x 4096: 110 / 91 / 72 / 96.
+// Splitting the depth costs 3 us and more, as long as all clusters run at once: 8 rows, 4096 x 1024: 20 us -> 11.5 with
+// eight blocks; 1024 x 1024: 7.9 -> 9.8.
+struct tile_cost {
+  int rows;
+  bool pair;
+  double stage, rest, store;
+};
+constexpr tile_cost kTmaCosts[4] = {{64, false, 0.275, 0.7, 1.3}, {128, false, 0.40, 0.9, 1.8}, {256, false, 0.47, 1.6, 2.8},
+                                    {256, true, 0.43, 1.6, 4.2}};
+constexpr tile_cost kLineCosts[3] = {{64, false, 1.45, 0.7, 1.3}, {128, false, 1.65, 0.9, 1.8}, {256, false, 2.1, 1.6, 2.8}};
+constexpr int kMostClusters[4] = {148, 72, 32, 12};   // of 1, 2, 4, 8 blocks, that are sure to run at once
+
+tile_choice choose_product(int64_t R, int64_t G, int64_t K, int64_t cols, bool tma) {
+  const double stages = (double)((K + kDepth - 1) / kDepth), groups = (double)std::min(R, G);
+  tile_choice best = {64, false, 1};
+  double least = 1e30;
+  for (int i = 0; i < (tma ? 4 : 3); ++i) {
+    const tile_cost& c = tma ? kTmaCosts[i] : kLineCosts[i];
+    if (c.pair && !wide_enough_for_pairs(cols)) continue;
+    const double width = c.pair ? 2 * kLanes : kLanes, across = std::ceil((double)cols / width);
+    const double tiles = across * std::max(groups, (double)R / c.rows + groups / 2);
+    const double t = std::ceil(tiles / (c.pair ? 74 : 148)) * std::max(c.store, stages * c.stage + c.rest);
+    if (t < least) best = {c.rows, c.pair, 1}, least = t;
+    for (int n = 1; i == 0 && n < 4 && stages >= 2 << n; ++n) {   // at least two stages to a block
+      const double split = stages / (1 << n) * c.stage + c.rest + 3 + 0.4 * n;
+      if (tiles <= kMostClusters[n] && split < least) best = {c.rows, false, 1 << n}, least = split;
+    }
+  }
+  return best;
+}
+
+// The choice for a gradient, whose depth is the rows of a group (or of a piece of one).  Tiles enough for the SMs: 256 rows,
+// pairs where there are about 512 rows to work on, below which a tile is little more than its stores (64 groups, 2048 x
+// 2048: 189 us against 229 for 6,000 rows; 4 groups of 750: 37 against 36).  Fewer tiles: smaller ones (one group of 600
+// rows, 1024 x 1024: 10.4 / 8.4 / 7.1 us with 256 / 128 / 64), and no larger than the output.  Without TMA 128 for twice as
+// many whole groups (30,000 rows of 4 groups, 1025 x 1023: 672 / 512 / 746 us with 64 / 128 / 256).
+tile_choice choose_gradient(int64_t R, int64_t G, int64_t I, int64_t J, const piece_plan& p, bool tma) {
+  const double pieces = (double)G + p.slots / 2;   // (about half of the slots are used)
+  const double tiles = pieces * (double)((I + 255) / 256) * (double)((J + kLanes - 1) / kLanes);
+  if (tiles < 50 || I <= 64) return {64, false, 1};
+  if (tiles < 100 || I <= 128 || (!tma && tiles < 200 && p.slots == 0)) return {128, false, 1};
+  return {256, wide_enough_for_pairs(J) && (double)R / pieces >= 512, 1};
+}
+
 // What a product is launched with.
 struct product_call {
   tensor_args a;
   CUtensorMap ma, mb;
   void* out;
-  bool wide, tma;
+  tile_choice tile;
+  bool tma;
   int64_t units;   // no more tiles than that
 };
 
-// Two blocks to a tile of 256 x 256: each fetches one half of either operand, 64 bytes for every 128 x 128 x 1 products where
-// a block alone fetches 96, more than the L2 cache delivers to all SMs at full speed.  Where the output is wide enough that its last
-// tile of 256 columns is not often half empty.
-bool pays_as_pair(int64_t cols) { return cols > kLanes && (cols >= 1024 || (cols - 1) % 256 >= 128); }
-
 template <typename T, int MODE, bool TMA>
 cudaError_t launch_product(hpspmm_ctx* ctx, const product_call& c, cudaStream_t s) {
-  if (TMA && c.wide && pays_as_pair(c.a.cols)) return launch_one<T, MODE, 256, 6, 1, true, true>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
-  if (c.wide) return launch_one<T, MODE, 256, 4, 1, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
-  const int stages = (c.a.depth + kDepth - 1) / kDepth;
-  int cl = 8;
-  while (cl > 1 && (c.units * cl > ctx->sm_count || stages < 2 * cl)) cl /= 2;
-  if (cl == 8) return launch_one<T, MODE, 64, 7, 8, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
-  if (cl == 4) return launch_one<T, MODE, 64, 7, 4, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
-  if (cl == 2) return launch_one<T, MODE, 64, 7, 2, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (TMA && c.tile.pair) return launch_one<T, MODE, 256, 6, 1, true, true>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (c.tile.rows == 256) return launch_one<T, MODE, 256, 4, 1, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (c.tile.rows == 128) return launch_one<T, MODE, 128, 6, 1, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (c.tile.blocks == 8) return launch_one<T, MODE, 64, 7, 8, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (c.tile.blocks == 4) return launch_one<T, MODE, 64, 7, 4, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
+  if (c.tile.blocks == 2) return launch_one<T, MODE, 64, 7, 2, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
   return launch_one<T, MODE, 64, 8, 1, TMA>(ctx, c.a, c.ma, c.mb, c.out, c.units, s);
 }
 template <typename T>
@@ -794,15 +855,13 @@ cudaError_t launch_product(hpspmm_ctx* ctx, const product_call& c, bool out_firs
   return out_first ? launch_product<T, MODE_OUT_FIRST, false>(ctx, c, s) : launch_product<T, MODE_IN_FIRST, false>(ctx, c, s);
 }
 
-template <typename T>
-cudaError_t launch_weight_grad(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* dW, bool tma,
-                               bool wide, int64_t units, cudaStream_t s) {
-  if (tma && wide && pays_as_pair(a.cols)) return launch_one<T, MODE_WEIGHT, 256, 6, 1, true, true>(ctx, a, ma, mb, dW, units, s);
-  if (tma)
-    return wide ? launch_one<T, MODE_WEIGHT, 256, 4, 1, true>(ctx, a, ma, mb, dW, units, s)
-                : launch_one<T, MODE_WEIGHT, 64, 8, 1, true>(ctx, a, ma, mb, dW, units, s);
-  return wide ? launch_one<T, MODE_WEIGHT, 256, 4, 1, false>(ctx, a, ma, mb, dW, units, s)
-              : launch_one<T, MODE_WEIGHT, 64, 8, 1, false>(ctx, a, ma, mb, dW, units, s);
+template <typename T, bool TMA>
+cudaError_t launch_weight_grad(hpspmm_ctx* ctx, const tensor_args& a, const CUtensorMap& ma, const CUtensorMap& mb, void* dW,
+                               const tile_choice& c, int64_t units, cudaStream_t s) {
+  if (TMA && c.pair) return launch_one<T, MODE_WEIGHT, 256, 6, 1, true, true>(ctx, a, ma, mb, dW, units, s);
+  if (c.rows == 256) return launch_one<T, MODE_WEIGHT, 256, 4, 1, TMA>(ctx, a, ma, mb, dW, units, s);
+  if (c.rows == 128) return launch_one<T, MODE_WEIGHT, 128, 6, 1, TMA>(ctx, a, ma, mb, dW, units, s);
+  return launch_one<T, MODE_WEIGHT, 64, 8, 1, TMA>(ctx, a, ma, mb, dW, units, s);
 }
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -813,23 +872,21 @@ int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t
                                   const void* W, bool out_first, const int32_t* offsets, void* Y, cudaStream_t s) {
   const bool half = type == HPSPMM_TYPE_F16;
   product_call c = {};
-  const int64_t across = (N + kLanes - 1) / kLanes;
-  // tiles of 256 rows where groups have more than 64 in the mean and the tiles (half a one more for each group) fill the SMs
-  c.wide = R > 64 * G && (R / 256 + G / 2) * across >= ctx->sm_count;
   c.out = Y;
-  const int64_t bn = c.wide ? 256 : 64;
-  if ((R / bn + G + 1) * across > kMaxTiles || R / bn + G + 1 > kMostTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
+  const int64_t across = (N + kLanes - 1) / kLanes;
+  if ((R / 64 + G + 1) * across > kMaxTiles || R / 64 + G + 1 > kMostTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
   const int64_t wsize[3] = {out_first ? K : N, out_first ? N : K, G}, wstride[2] = {wsize[0], K * N};
   const int wbox[3] = {64, out_first ? kLanes : kDepth, 1};
   const int64_t xsize[2] = {K, R}, xstride[1] = {ldx};
-  const int xbox[2] = {kDepth, c.wide ? box_rows<256>() : box_rows<64>()};
+  const int xbox[2] = {kDepth, 64};
   c.tma = K % 8 == 0 && N % 8 == 0 && ldx % 8 == 0 && ldx >= K && aligned(X) && aligned(W) && aligned(Y) &&
           encode(&c.ma, half, W, 3, wsize, wstride, wbox) && encode(&c.mb, half, X, 2, xsize, xstride, xbox);
+  c.tile = choose_product(R, G, K, N, c.tma);
   for (int64_t g0 = 0; g0 < G; g0 += kMaxGroups) {
     const int64_t gn = std::min<int64_t>(kMaxGroups, G - g0);
     c.a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, {(int)R, 0}, nullptr,
            ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS, W, X, wsize[0], ldx};
-    c.units = (std::min(R, gn) + R / bn) * across;
+    c.units = (std::min(R, gn) + R / c.tile.rows) * across;
     HPSPMM_CUDA_TRY(ctx, half ? launch_product<__half>(ctx, c, out_first, s) : launch_product<__nv_bfloat16>(ctx, c, out_first, s));
   }
   return HPSPMM_OK;
@@ -840,19 +897,22 @@ int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int
                                       int64_t lda, const void* B, int64_t ldb, const int32_t* offsets, void* dW,
                                       const piece_plan& p, float* slots, cudaStream_t s) {
   const bool half = type == HPSPMM_TYPE_F16;
-  const int64_t across = (J + kLanes - 1) / kLanes;
-  const bool wide = (G + p.slots / 2) * ((I + 255) / 256) * across >= ctx->sm_count;   // (about half of the slots are used)
-  const int64_t bn = wide ? 256 : 64, units = (G + p.slots) * ((I + bn - 1) / bn) * across;
-  if (units > kMaxTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
   CUtensorMap ma = {}, mb = {};   // the operand of the output's columns lies on the lanes
   const int64_t asize[2] = {J, R}, astride[1] = {ldb}, bsize[2] = {I, R}, bstride[1] = {lda};
   const int box[2] = {64, kDepth};
   const bool tma = I % 8 == 0 && J % 8 == 0 && lda % 8 == 0 && ldb % 8 == 0 && lda >= I && ldb >= J && aligned(A) && aligned(B) &&
                    encode(&ma, half, B, 2, asize, astride, box) && encode(&mb, half, A, 2, bsize, bstride, box);
+  const tile_choice c = choose_gradient(R, G, I, J, p, tma);
+  const int64_t units = (G + p.slots) * ((I + c.rows - 1) / c.rows) * ((J + kLanes - 1) / kLanes);
+  if (units > kMaxTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
   const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, p, slots, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS,
                          B, A, ldb, lda};
-  const cudaError_t e = half ? launch_weight_grad<__half>(ctx, a, ma, mb, dW, tma, wide, units, s)
-                             : launch_weight_grad<__nv_bfloat16>(ctx, a, ma, mb, dW, tma, wide, units, s);
+  cudaError_t e;
+  if (half)
+    e = tma ? launch_weight_grad<__half, true>(ctx, a, ma, mb, dW, c, units, s) : launch_weight_grad<__half, false>(ctx, a, ma, mb, dW, c, units, s);
+  else
+    e = tma ? launch_weight_grad<__nv_bfloat16, true>(ctx, a, ma, mb, dW, c, units, s)
+            : launch_weight_grad<__nv_bfloat16, false>(ctx, a, ma, mb, dW, c, units, s);
   HPSPMM_CUDA_TRY(ctx, e);
   return HPSPMM_OK;
 }

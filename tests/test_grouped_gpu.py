@@ -366,3 +366,15 @@ def test_streams_and_threads_at_once(ops):
         t.join()
     assert not errors, errors[0]
     assert ops.timeouts() == 0
+
+
+@pytest.mark.parametrize("K", [8, 64, 120, 128, 130, 256, 328, 403, 512, 520, 777, 1000, 1024, 2049, 4096])
+def test_few_rows_of_every_depth(ops, K):
+    """A step of a decoder: blocks that split the depth of one tile, where it is long enough for that."""
+    gen = torch.Generator("cuda").manual_seed(K)
+    for dtype in (torch.float16, torch.bfloat16):
+        for sizes in ([1], [3, 2], [0, 17, 0, 5], [40, 1, 60]):
+            for N in (8, 22, 136):
+                X, dY = (torch.randn((sum(sizes) + 2, c), device="cuda", generator=gen).to(dtype) for c in (K, N))
+                for transposed in (False, True):
+                    _check(ops, X, _weights(len(sizes), K, N, dtype, gen, transposed), _offsets(sizes), dY)
