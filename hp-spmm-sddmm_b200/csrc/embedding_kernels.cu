@@ -436,7 +436,8 @@ struct backward_plan {
   size_t keys, pos, tables, info, split, bytes;   // offsets
 };
 
-// Places to a part: 16 to 256, as many as leave 48 warps for every SM (a slab of columns is 256 wide at least).  Longer
+// Places to a part: 16 to 256, as many as leave 64 warps for every SM, two rounds of them (16,384 positions of 131,072 x
+// 1024: 58 us, with 32 warps 65; a slab of columns is taken to be 256 wide).  Longer
 // parts mean fewer rows in several of them: 64 instead of 256 cost 53 us instead of 17 in the join for 262,144 positions of
 // 262,144 x 2048.
 backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
@@ -450,7 +451,7 @@ backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
   if (T > 1 << 20) p.chunk = (T + 147) / 148;
   p.chunk = std::max<int64_t>(1, (p.chunk + kSortThreads - 1) / kSortThreads) * kSortThreads;
   p.blocks = (int)((T + p.chunk - 1) / p.chunk);
-  p.length = (int)std::min<int64_t>(256, std::max<int64_t>(16, ((T + N) * ((K + 255) / 256) / (148 * 48) + 15) / 16 * 16));
+  p.length = (int)std::min<int64_t>(256, std::max<int64_t>(16, ((T + N) * ((K + 255) / 256) / (148 * 64) + 15) / 16 * 16));
   p.parts = (T + N + p.length - 1) / p.length;
   const size_t b_t = align_up((size_t)T * 4, 256);
   p.keys = 0;
