@@ -410,6 +410,7 @@ int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int
     HPSPMM_CUDA_TRY(ctx, cudaMemsetAsync(Y, 0, (size_t)(R * N) * dense_type_size(type), s));
     return HPSPMM_OK;
   }
+  if (type != HPSPMM_TYPE_F32 && K > kMostDepth) return hpspmm_unsupported(ctx, "16-bit products deeper than 2^27");
   if (type != HPSPMM_TYPE_F32)
     return hpspmm_grouped_product_tensor(ctx, R, G, K, N, type, X, ldx, W, w_out_first != 0, offsets, Y, s);
   if (((R + kProductRows - 1) / kProductRows + G + 2) * ((N + 63) / 64) > 2147483647ll)
@@ -466,6 +467,7 @@ int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K,
     HPSPMM_REQUIRE(ctx, ((uintptr_t)workspace & 255) == 0, "workspace not aligned to 256 bytes");
   }
   if (type != HPSPMM_TYPE_F32) {
+    if (p.length > kMostDepth) return hpspmm_unsupported(ctx, "16-bit gradients over more than 2^27 rows that are not cut into pieces");
     const int done = hpspmm_grouped_weight_grad_tensor(ctx, R, G, I, J, type, A, lda, B, ldb, offsets, dW, p, slots, s);
     if (done != HPSPMM_OK) return done;
   } else {

@@ -268,6 +268,12 @@ def test_refusals(ops, pkg, gpu_ctx):
     for at, v in ((0, -1), (4, -1), (5, None), (6, -1), (7, None), (8, -1), (9, None), (10, None), (1, 1 << 40)):
         with pytest.raises(pkg.HpspmmError):
             gpu_ctx.grouped_weight_grad(*(good[:at] + [v] + good[at + 1:]))
+    with pytest.raises(pkg.HpspmmError, match="2\\^27"):
+        gpu_ctx.grouped_product(6, 2, (1 << 27) + 8, 4, pkg.TYPE_BF16, X.data_ptr(), (1 << 27) + 8, W.data_ptr(), 0, off.data_ptr(),
+                                Y.data_ptr())
+    with pytest.raises(pkg.HpspmmError, match="2\\^27"):
+        gpu_ctx.grouped_weight_grad((1 << 27) + 1, 3000, 8, 4, pkg.TYPE_BF16, X.data_ptr(), 8, Y.data_ptr(), 4, off.data_ptr(),
+                                    W.data_ptr(), 0)
     size = pkg.load_library().hpspmm_grouped_weight_grad_workspace
     for dtype in (pkg.TYPE_F32, pkg.TYPE_BF16):
         assert size(0, 3, 8, 8, dtype, 0) == 0 and size(100, 3, 8, 8, dtype, 1) == 0
