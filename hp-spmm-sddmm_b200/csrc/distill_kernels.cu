@@ -16,7 +16,10 @@ using namespace hpspmm;
 
 constexpr int kThreads = 256;
 constexpr int kMaxEntries = 1024;   // of the teacher for one row
-constexpr int kMaxEntriesWarp = 64; // where a warp has a row
+// Entries that a row has room for in shared memory: 1024 to a block; to a warp 64, or 256 for teachers of more (20,000 rows of
+// 2,048 bf16 and 64 entries: forward and gradient 94 us with room for 64, 111 for 256).
+constexpr int kFewEntriesWarp = 64;
+constexpr int kMaxEntriesWarp = 256;
 // Vectors of 16 bytes in flight per thread.  4,096 x 131,072 bf16: backward 357 us with four, 346 with eight; forward with
 // four 185 us where six blocks to an SM are asked for, 196 without (1,021 x 32,003 floats: 39 and 32).
 constexpr int kForwardVectors = 4;
@@ -102,13 +105,13 @@ struct running {
 
 // One pass over the row, everything in registers: NT threads to a row, CL blocks of a cluster to one where rows are few.
 // Bound by the reads of the logits; an element costs one ex2 and about five other instructions.
-template <typename T, int NT, int CL>
+template <typename T, int NT, int CL, int ENTRIES>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 0)
 distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
                        const float* __restrict__ teacher, float tau, float* __restrict__ loss, float2* __restrict__ stats) {
   typedef dense_vec<T, 16> vec;
   constexpr int E = vec::kCount, kTogether = 8 / E;   // eight values to a step
-  constexpr int kRows = kThreads / NT, kEntries = NT == 32 ? kMaxEntriesWarp : kMaxEntries;
+  constexpr int kRows = kThreads / NT, kEntries = ENTRIES;
   __shared__ float of_teacher[kRows][kEntries], of_student[kRows][kEntries];   // logits at the teacher's entries
   __shared__ float part[kThreads / 32];
   __shared__ float2 from_rank[CL];
@@ -201,14 +204,14 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
 
 // One read and one write of the row; the columns that the teacher names are written again by the first of their entries.
 // slices: blocks to a row where rows are few.  The last rows come first: the forward pass left them in the L2 cache.
-template <typename T, int NT>
+template <typename T, int NT, int ENTRIES>
 __global__ void __launch_bounds__(kThreads)
 distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
                         const float* __restrict__ teacher, float tau, const float2* __restrict__ stats,
                         const float* __restrict__ dloss, int64_t dloss_stride, T* __restrict__ dlogits, int slices) {
   typedef dense_vec<T, 16> vec;
   constexpr int E = vec::kCount;
-  constexpr int kRows = kThreads / NT, kEntries = NT == 32 ? kMaxEntriesWarp : kMaxEntries;
+  constexpr int kRows = kThreads / NT, kEntries = ENTRIES;
   __shared__ int id_of[kRows][kEntries];
   __shared__ float p_of[kRows][kEntries], part[kThreads / 32];
   const int tid = threadIdx.x & (NT - 1), slot = NT == 32 ? threadIdx.x >> 5 : 0;
@@ -309,7 +312,7 @@ cudaError_t launch_cluster(int64_t rows, int V, int k, const void* logits, int64
   attr.val.clusterDim.x = CL, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3((unsigned)(rows * CL)), c.blockDim = dim3(kThreads), c.stream = s, c.attrs = &attr, c.numAttrs = CL > 1;
-  return cudaLaunchKernelEx(&c, distill_forward_kernel<T, kThreads, CL>, rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, loss,
+  return cudaLaunchKernelEx(&c, distill_forward_kernel<T, kThreads, CL, kMaxEntries>, rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, loss,
                             (float2*)stats);
 }
 
@@ -318,8 +321,8 @@ cudaError_t launch_forward(hpspmm_ctx* ctx, int64_t rows, int V, int k, const vo
                            const float* teacher, float tau, float* loss, float* stats, cudaStream_t s) {
   const distill_shape sh = choose_distill(ctx, rows, V, k, (int)sizeof(T));
   if (sh.warp) {
-    distill_forward_kernel<T, 32, 1><<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher,
-                                                                                    tau, loss, (float2*)stats);
+    auto* kernel = k <= kFewEntriesWarp ? distill_forward_kernel<T, 32, 1, kFewEntriesWarp> : distill_forward_kernel<T, 32, 1, kMaxEntriesWarp>;
+    kernel<<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, loss, (float2*)stats);
     return cudaSuccess;
   }
   if (sh.parts == 8) return launch_cluster<T, 8>(rows, V, k, logits, ld, ids, wide, teacher, tau, loss, stats, s);
@@ -333,12 +336,11 @@ void launch_backward(hpspmm_ctx* ctx, int64_t rows, int V, int k, const void* lo
                      const float* teacher, float tau, const float* stats, const float* dloss, int64_t stride, void* dlogits,
                      cudaStream_t s) {
   const distill_shape sh = choose_distill(ctx, rows, V, k, (int)sizeof(T));
-  if (sh.warp)
-    distill_backward_kernel<T, 32><<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(
-        rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, (const float2*)stats, dloss, stride, (T*)dlogits, 1);
-  else
-    distill_backward_kernel<T, kThreads><<<(unsigned)(rows * sh.parts), kThreads, 0, s>>>(
-        rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, (const float2*)stats, dloss, stride, (T*)dlogits, sh.parts);
+  auto* kernel = !sh.warp ? distill_backward_kernel<T, kThreads, kMaxEntries>
+                          : (k <= kFewEntriesWarp ? distill_backward_kernel<T, 32, kFewEntriesWarp> : distill_backward_kernel<T, 32, kMaxEntriesWarp>);
+  const int64_t blocks = sh.warp ? (rows + 7) / 8 : rows * sh.parts;
+  kernel<<<(unsigned)blocks, kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, (const float2*)stats, dloss, stride,
+                                               (T*)dlogits, sh.parts);
 }
 
 int check_distill(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int32_t type, int64_t ld, int32_t id_bytes, float tau) {

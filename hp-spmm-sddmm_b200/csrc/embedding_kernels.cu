@@ -436,10 +436,11 @@ struct backward_plan {
   size_t keys, pos, tables, info, split, bytes;   // offsets
 };
 
-// Places to a part: 16 to 256, as many as leave 64 warps for every SM, two rounds of them (16,384 positions of 131,072 x
-// 1024: 58 us, with 32 warps 65; a slab of columns is taken to be 256 wide).  Longer
-// parts mean fewer rows in several of them: 64 instead of 256 cost 53 us instead of 17 in the join for 262,144 positions of
-// 262,144 x 2048.
+// Places to a part: 16 to 256, as many as leave 64 warps for every SM, two rounds of them, with slabs of 256 columns (16,384
+// positions of 131,072 x 1024: 58 us, with 32 warps 65).  Longer parts mean fewer rows in several of them: 64 instead of 256
+// cost 53 us instead of 17 in the join for 262,144 positions of 262,144 x 2048.  (Narrow rows, four groups of lanes to a
+// warp, would sum faster in shorter parts, but their join takes more than that: 3 M positions, 16 columns 104 + 83 against
+// 140 + 28 us.)
 backward_plan plan_backward(int64_t T, int64_t N, int64_t K) {
   backward_plan p = {};
   while (p.bits < 31 && ((int64_t)1 << p.bits) <= N) ++p.bits;
@@ -536,11 +537,14 @@ template <typename T, int BYTES>
 void launch_lookup(int64_t T_, int64_t N, int64_t K, const void* ids, int wide, const void* table, int64_t ld, float scale, void* out,
                    cudaStream_t s) {
   const int per_row = (int)(K * (int64_t)sizeof(T) / BYTES);
-  // rows of up to 32 vectors: 8 lanes with up to four each, so that as much is in flight as with wide rows
-  const int W = per_row <= 32 ? 8 : 32;
+  // rows of up to 32 (8) vectors: 8 (2) lanes with up to four each, so that as much is in flight as with wide rows
+  const int W = per_row <= 8 ? 2 : (per_row <= 32 ? 8 : 32);
   const int64_t pieces = (per_row + 4 * W - 1) / (4 * W), groups = T_ * pieces;
   const dim3 grid((unsigned)((groups * W + kThreads - 1) / kThreads));
-  if (W == 8)
+  if (W == 2)
+    hpspmm_launch(lookup_kernel<T, BYTES, 2>, grid, dim3(kThreads), 0, s, groups, (int)pieces, per_row, (int)N, ids, wide, (const T*)table, ld,
+                  scale, (T*)out);
+  else if (W == 8)
     hpspmm_launch(lookup_kernel<T, BYTES, 8>, grid, dim3(kThreads), 0, s, groups, (int)pieces, per_row, (int)N, ids, wide, (const T*)table, ld,
                   scale, (T*)out);
   else

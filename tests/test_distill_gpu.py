@@ -360,3 +360,30 @@ print("well")
 """ % (root, os.path.join(root, "tests"))
     out = subprocess.run([sys.executable, "-c", code], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip().endswith("well"), out.stdout[-2000:]
+
+
+def test_a_compiled_step_is_the_same(ops):
+    """Through the tracer and PyTorch's ahead-of-time autograd: same loss, same gradients."""
+    gen = torch.Generator("cuda").manual_seed(13)
+    ids, top = (torch.randint(-1, n, shape, device="cuda", generator=gen) for n, shape in ((50, (300,)), (32, (300, 4))))
+    table = torch.randn((50, 64), device="cuda", generator=gen).bfloat16().requires_grad_()
+    W = torch.randn((2, 32, 64), device="cuda", generator=gen).bfloat16().transpose(1, 2).requires_grad_()
+    offsets, teacher = torch.tensor([0, 100, 290], dtype=torch.int32, device="cuda"), torch.randn((300, 4), device="cuda", generator=gen)
+
+    def step(ids, table, W):
+        z = ops.grouped_product(ops.embedding(ids, table, 2.0), W, offsets)
+        return ops.topk_distill_loss(z, top, teacher, 2.0).mean()
+
+    first = step(ids, table, W)
+    grads = torch.autograd.grad(first, (table, W))
+    loss = torch.compile(step, backend="aot_eager", fullgraph=True)(ids, table, W)
+    assert torch.equal(loss, first)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(loss, (table, W))))
+
+
+@pytest.mark.parametrize("k", [63, 64, 65, 255, 256, 257, 1023])
+def test_short_rows_and_long_teachers(ops, k):
+    """Rows that a warp takes, with room for 64 or 256 entries, and rows that need a block for their entries alone."""
+    gen = torch.Generator("cuda").manual_seed(k)
+    for dtype in (torch.float32, torch.bfloat16):
+        _check(ops, *_inputs(37, 1024, k, dtype, gen), 1.3)

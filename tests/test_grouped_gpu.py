@@ -384,3 +384,25 @@ def test_few_rows_of_every_depth(ops, K):
                 X, dY = (torch.randn((sum(sizes) + 2, c), device="cuda", generator=gen).to(dtype) for c in (K, N))
                 for transposed in (False, True):
                     _check(ops, X, _weights(len(sizes), K, N, dtype, gen, transposed), _offsets(sizes), dY)
+
+
+def test_beside_the_librarys_products(ops):
+    """Kernels of another owner on the same tensor cores, on another stream: nobody waits for anybody."""
+    gen = torch.Generator("cuda").manual_seed(14)
+    X, W = torch.randn((3000, 1024), device="cuda", generator=gen).bfloat16(), _weights(4, 1024, 1024, torch.bfloat16, gen, False)
+    off, A = _offsets([500, 10, 1490, 1000]), torch.randn((2048, 2048), device="cuda", generator=gen).bfloat16()
+    want, tol = ref.grouped(X, W, off)
+    want_w, tol_w = ref.grouped_weight(X, X, off)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(40):
+        with torch.cuda.stream(one):
+            y = ops.grouped_product(X, W, off)
+            few = ops.grouped_product(X[:8], W, off // 400)
+        with torch.cuda.stream(two):
+            A @ A
+            dw = torch.ops.hpspmm.grouped_weight_grad(X, X, off, False)
+    torch.cuda.synchronize()
+    assert ref.outside(y, want, tol) == 0 and ref.outside(dw, want_w, tol_w) == 0 and ops.timeouts() == 0
+    want, tol = ref.grouped(X[:8], W, off // 400)
+    assert ref.outside(few, want, tol) == 0
