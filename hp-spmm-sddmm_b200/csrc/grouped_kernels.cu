@@ -85,7 +85,7 @@ __device__ __forceinline__ row_tile find_row_tile(const int* offsets, int G, int
 //
 // A tile of TR x BN outputs to a block of 2 TR threads, 8 x BN / 16 of them to a thread, in 32 bits from the operands on;
 // 16 of the depth at a time, copied asynchronously into a ring of three buffers in the order in which they lie in memory.
-// Bound by the multiply-adds, two of which go as one packed instruction (fma.rn.f32x2): on two neighbouring columns of the
+// Bound by the multiply-adds (60 % of the pipe's cycles for 100,003 rows of 47 groups, 100 x 64), two of which go as one packed instruction (fma.rn.f32x2): on two neighbouring columns of the
 // output, or, where both operands lie along the depth, on two neighbours of it, whose sums meet at the end.
 // TR = 64 for products, whose depth is short as often as not, so that more blocks hide each other's beginnings (100,003 x 100
 // by 47 matrices of 64: 46 us with 128, 41 with 64); 128 for gradients, which read less that way (55 us with 64, 46 with 128).
@@ -345,11 +345,12 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int64_t tile_columns(int64_t cols) { return cols <= 64 ? 64 : 128; }
 
 // Rows to a piece: all of them, or as many as fill the GPU once where that is expected to be faster.  In us: what 64 rows
-// take a tile (0.30 to 0.47 on the tensor cores, less with fewer tiles, which are smaller then, 1.65 without TMA; 9.6 or, 64 columns wide, 4.8
-// on the ordinary ones, which run two of them on an SM); whole groups take as long as the largest one, for which twice the
-// mean is assumed; pieces have at least 1024 (256) rows, take another launch and the way of their sums to memory and back
-// (4 TB/s; somewhat more than half of the slots are used).  16 groups of 750 rows, 1024 x 1024: 73 us in pieces, 31 whole; one group of 12,000, 4096 x 512: 59 us in pieces,
-// 71 whole; in 32 bits 16 groups of 750 rows, 512 x 512: 175 us in pieces, 270 whole.
+// take a tile (0.30 to 0.47 on the tensor cores, less with fewer tiles, which are smaller then, 1.65 without TMA; 9.6 or, 64
+// columns wide, 4.8 on the ordinary ones, which run two of them on an SM); whole groups take as long as the largest one,
+// for which twice the mean is assumed; pieces have at least 1024 (256) rows, take another launch and the way of their sums
+// to memory and back (4 TB/s; somewhat more than half of the slots are used).  16 groups of 750 rows, 1024 x 1024: 73 us in
+// pieces, 31 whole; one group of 12,000, 4096 x 512: 59 us in pieces, 71 whole; in 32 bits 16 groups of 750 rows, 512 x
+// 512: 175 us in pieces, 270 whole.
 piece_plan plan_pieces(int64_t R, int64_t G, int64_t I, int64_t J, int32_t type) {
   const bool f32 = type == HPSPMM_TYPE_F32;
   const int64_t bi = f32 ? kGradientRows : 256, bj = f32 ? tile_columns(J) : 128, least = f32 ? 256 : 1024;
