@@ -61,6 +61,10 @@ __device__ __forceinline__ void row_sync() {
 template <int NT>
 __device__ __forceinline__ bool row_any(bool v) { return NT == 32 ? __any_sync(0xffffffffu, v) : __syncthreads_or(v); }
 
+// of the blocks of a cluster
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // A row of V elements at any address: `head` elements in front of the first 16-byte boundary, vectors, the rest from `tail` on.
 template <typename T>
 struct row_parts {
@@ -120,6 +124,9 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
   const int rank = CL == 1 ? 0 : blockIdx.x & (CL - 1);
   const int64_t row = CL == 1 ? (int64_t)blockIdx.x * kRows + slot : blockIdx.x / CL;
   if (row >= rows) return;              // whole warps, and none of them in front of a barrier of the block
+  // a block may write into another one's shared memory only once that one is known to run: each says so here, and waits for
+  // the others behind its reads of the row
+  if (CL > 1) cluster_arrive();
   const T* z = logits + row * ld;
   const float c = kLog2e / tau;
   if (rank == 0)
@@ -160,13 +167,14 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
   float top = row_reduce<NT>(r.top, maximum(), part);
   float total = row_reduce<NT>(r.under(top, c), sum(), part);
   if (CL > 1) {   // the blocks' parts, in the order of their ranks
+    cluster_wait();
     if (threadIdx.x == 0) {
       uint32_t to;
       asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&from_rank[rank])));
       asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(top), "f"(total) : "memory");
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
     if (rank != 0) return;
     float most = -INFINITY;
 #pragma unroll
@@ -292,7 +300,7 @@ distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits
   }
 }
 
-// A warp to a row where rows are short; several blocks, each with at least 32 KB of it, to a row where the rows do not fill
+// A warp to a row where rows are short; several blocks, each with at least 16 KB of it, to a row where the rows do not fill
 // the SMs twice.  (Two or four to a row for more rows than that lost: 1,021 rows of 32,003 floats 32 us with one, 44 with
 // four: what a row costs beside its reads comes with every block.)
 struct distill_shape {

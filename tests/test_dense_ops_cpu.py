@@ -41,3 +41,26 @@ def test_workspace_sizes(pkg):
         got = need(T, 100_000, 64)
         assert got >= 8 * T and got >= last
         last = got
+
+
+def test_no_block_writes_into_a_cluster_before_all_of_it_runs():
+    """A block that has not started has no shared memory to write into: in every kernel that stores into another block's, a
+    wait for the cluster comes first.  (Nothing else shows its absence: the blocks of a cluster mostly start together.)"""
+    import glob
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hp-spmm-sddmm_b200", "csrc")
+    seen = 0
+    for path in sorted(glob.glob(os.path.join(csrc, "*.cu"))):
+        source = re.sub(r"//[^\n]*", "", open(path).read())
+        for kernel in source.split("__global__")[1:]:
+            body = kernel[:kernel.index("\n}\n")]
+            store = re.search(r"st\.shared::cluster", body)
+            if store:
+                seen += 1
+                before = body[:store.start()]
+                waits = [before.find(x) for x in ("cluster_wait()", "barrier.cluster.wait")]
+                arrives = [before.find(x) for x in ("cluster_arrive()", "barrier.cluster.arrive")]
+                assert max(waits) >= 0 and max(arrives) >= 0, path
+                assert min(x for x in arrives if x >= 0) < min(x for x in waits if x >= 0), path
+    assert seen == 2

@@ -387,3 +387,25 @@ def test_short_rows_and_long_teachers(ops, k):
     gen = torch.Generator("cuda").manual_seed(k)
     for dtype in (torch.float32, torch.bfloat16):
         _check(ops, *_inputs(37, 1024, k, dtype, gen), 1.3)
+
+
+@pytest.mark.parametrize("T", [1, 5, 37, 140])
+def test_few_long_rows_again_and_again_on_a_busy_gpu(ops, T):
+    """Clusters whose blocks find their SMs at different times, beside products on another stream: the same bits every time."""
+    gen = torch.Generator("cuda").manual_seed(20 + T)
+    z, ids, teacher = _inputs(T, 40_000, 9, torch.bfloat16, gen)
+    A = torch.randn((2048, 2048), device="cuda", generator=gen).bfloat16()
+    want, tol = ref.distill(z, ids, teacher, 1.0)
+    first = torch.ops.hpspmm.topk_distill(z, ids, teacher, 1.0)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    held = []
+    for _ in range(60):
+        with torch.cuda.stream(two):
+            A @ A
+        with torch.cuda.stream(one):
+            held.append(torch.ops.hpspmm.topk_distill(z, ids, teacher, 1.0))
+    torch.cuda.synchronize()
+    assert ref.outside(first[0], want, tol) == 0
+    for loss, stats in held:
+        assert torch.equal(loss, first[0]) and torch.equal(stats, first[1])
