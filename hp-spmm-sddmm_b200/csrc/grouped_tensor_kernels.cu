@@ -16,6 +16,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "dense_types.cuh"
@@ -49,6 +50,8 @@ struct tensor_args {
   // the operands on the lanes and on the N side, for calls whose tiles TMA cannot fetch: rows ld elements apart
   const void *a, *b;
   int64_t lda, ldb;
+  long long wait_limit;   // cycles
+  int withhold;           // (for tests) nothing is copied, so that the waits for the copies run out
 };
 
 // ---- instructions ------------------------------------------------------------------------------------------------
@@ -85,22 +88,42 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity), "r"(kSleep) : "memory");
   return ok != 0;
 }
-// Waits for at most about two seconds.  Whoever gives up says so in `failed`, and all others give up with it.
-template <bool CLUSTER>
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* failed) {
+// What the waits of a block share.
+struct wait_state {
+  int failed;          // one of them has been given up, so all others are
+  long long limit;     // cycles that one may take
+};
+// By one thread.  Whoever gives up says so in `failed`, and all others give up with it.
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile wait_state* w) {
   const long long begin = clock64();
   while (true) {
-    if (mbar_try<CLUSTER>(bar, parity)) return true;
-    if (*failed) return false;
-    if (clock64() - begin > 4000000000ll) {
-      *failed = 1;
+    if (mbar_try<false>(bar, parity)) return true;
+    if (w->failed) return false;
+    if (clock64() - begin > w->limit) {
+      w->failed = 1;
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile wait_state* w) {
+  return mbar_try<false>(bar, parity) || mbar_wait_slow(bar, parity, w);
+}
+// By a whole warp, with the same answer in all lanes: what follows are instructions that all of them have to reach, so that
+// lanes which gave up while others did not would leave those waiting for good.
+template <bool CLUSTER>
+__device__ __noinline__ bool mbar_wait_warp_slow(uint32_t bar, uint32_t parity, volatile wait_state* w) {
+  const long long begin = clock64();
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_try<CLUSTER>(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, w->failed || clock64() - begin > w->limit)) {
+      w->failed = 1;
       return false;
     }
   }
 }
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
-  return mbar_try<CLUSTER>(bar, parity) || mbar_wait_slow<CLUSTER>(bar, parity, failed);
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile wait_state* w) {
+  return __all_sync(0xffffffffu, mbar_try<CLUSTER>(bar, parity)) || mbar_wait_warp_slow<CLUSTER>(bar, parity, w);
 }
 
 // PAIR: the barrier may be the one of the pair's other block (`bar` is an address in the cluster's window)
@@ -344,7 +367,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   __shared__ int part[kThreads / 32];
   __shared__ uint64_t bars[4 * STAGES + 6];
   __shared__ uint32_t tmem_base;
-  __shared__ int failed;
+  __shared__ wait_state waits;
   const uint32_t base = (smem_of(raw) + 1023) / 1024 * 1024;
   const uint32_t bar0 = smem_of(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
@@ -360,7 +383,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   if (kBlocks > 1) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
 
   if (threadIdx.x == 0) {
-    failed = 0;
+    waits.failed = 0, waits.limit = a.wait_limit;
     for (int s = 0; s < STAGES; ++s) mbar_init(full(s), TMA ? 1 : kLoaders), mbar_init(empty(s), 1), mbar_init(cleared(s), PAIR ? 2 : 1), mbar_init(cut_full(s), 1);
     for (int b = 0; b < 2; ++b) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), PAIR ? 8 : 4);
     mbar_init(parts_full, 4 * CL), mbar_init(parts_empty, 4 * CL);
@@ -426,7 +449,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   const int first = blockIdx.x / kBlocks, step = gridDim.x / kBlocks;
 
   if (warp == 0) {
-    if (TMA && lane == 0) {   // copies
+    if (TMA && lane == 0 && !a.withhold) {   // copies
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -437,7 +460,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         const int from = t.row0 + (PAIR ? rank * half : 0), count = PAIR ? half : t.rows;
         const int boxes = (count + 63) / 64;
         for (int k = 0; k < t.stages; ++k) {
-          ok = mbar_wait(empty(s), phase ^ 1, &failed);
+          ok = mbar_wait(empty(s), phase ^ 1, &waits);
           if (!ok) break;
           // The copies of both blocks of a pair arrive at the first one's barrier.  A stage that is cut short has a barrier of
           // its own, in either block: its rest has to be cleared before it is used.
@@ -494,7 +517,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       look_up(first);
       for (int u = first; u < units && ok; u += step) {
         w = next;
-        ok = mbar_wait<PAIR>(acc_empty(acc), acc_phase ^ 1, &failed);
+        ok = mbar_wait_warp<PAIR>(acc_empty(acc), acc_phase ^ 1, &waits);
         if (!ok) break;
         tensor_fence_after();
         const uint32_t d = tmem + acc * BN;
@@ -505,10 +528,10 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         for (int k = 0; k < w.stages; ++k) {
           const bool last = k + 1 == w.stages;
           if (last && w.cut) {
-            ok = mbar_wait<PAIR>(cleared(s), cut_phase >> s & 1, &failed);
+            ok = mbar_wait_warp<PAIR>(cleared(s), cut_phase >> s & 1, &waits);
             cut_phase ^= 1u << s;
           } else {
-            ok = mbar_wait(full(s), full_phase >> s & 1, &failed);
+            ok = mbar_wait_warp(full(s), full_phase >> s & 1, &waits);
             full_phase ^= 1u << s;
           }
           if (!ok) break;
@@ -550,7 +573,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       if (t.stages == 0) continue;
       s = (s + t.stages - 1) % STAGES;
       if (cut_short(t, t.stages - 1)) {
-        if (!mbar_wait(cut_full(s), phase >> s & 1, &failed)) break;
+        if (!mbar_wait_warp(cut_full(s), phase >> s & 1, &waits)) break;
         phase ^= 1u << s;
         const uint32_t src = base + s * kStage;
         const int left = t.end - t.begin - (t.stages - 1) * kDepth;
@@ -574,7 +597,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     int s = 0, turn = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int u = first; u < units && ok; u += step) {
+    for (int u = a.withhold ? units : first; u < units && ok; u += step) {
       const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
       for (int k = 0; k < t.stages; ++k) {
         const int at = s;
@@ -582,7 +605,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
         if (++s == STAGES) s = 0, phase ^= 1;
         turn = turn + 1 == kTeams ? 0 : turn + 1;
         if (turn != team) continue;
-        ok = mbar_wait(empty(at), parity, &failed);
+        ok = mbar_wait_warp(empty(at), parity, &waits);
         if (!ok) break;
         const uint32_t dst = base + at * kStage;
         if (kWeight) {
@@ -613,7 +636,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     if (CL > 1) cluster_wait();
     for (int u = first; u < units; u += step) {
       const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
-      if (!mbar_wait(acc_full(acc), acc_phase, &failed)) break;
+      if (!mbar_wait_warp(acc_full(acc), acc_phase, &waits)) break;
       tensor_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(q * 32) << 16);
       const int col = t.col0 + q * 32 + lane;
@@ -653,7 +676,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       } else {
         // Every block takes 1 / CL of the tile's rows and gets the others' parts of them pushed into its shared memory.
         const int share = (t.rows + 15) / 16 * 16 / CL;
-        if (!mbar_wait<true>(parts_empty, part_phase ^ 1, &failed)) break;
+        if (!mbar_wait_warp<true>(parts_empty, part_phase ^ 1, &waits)) break;
         const uint32_t mine = smem_of(parts + rank * share * kLanes + q * 32 + lane);
         int to_rank = 0, r = 0;
         uint32_t at = in_block(mine, 0);
@@ -679,7 +702,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
           for (int p = 0; p < CL; ++p) mbar_arrive_remote(parts_full, p);
         }
         __syncwarp();
-        if (!mbar_wait<true>(parts_full, part_phase, &failed)) break;
+        if (!mbar_wait_warp<true>(parts_full, part_phase, &waits)) break;
         for (int r = 0; r < share; ++r) {
           float sum = 0.f;
 #pragma unroll
@@ -708,10 +731,11 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   }
   tensor_fence_before();
   __syncthreads();
-  if (failed) {   // what was started lands before the memory is given back
+  if (waits.failed) {   // what was started lands before the memory is given back
     if (threadIdx.x == 0) atomicAdd(a.timeouts, 1);
     const long long begin = clock64();
     while (clock64() - begin < 4000000ll) __nanosleep(1000);
+    __syncwarp();
   }
   if (kBlocks > 1) {   // nobody reaches into the memory of a block that has left
     if (CL > 1 && (warp < 4 || warp >= kThreads / 32)) cluster_wait();
@@ -726,6 +750,11 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
+
+// Of a wait, in cycles: about two seconds.  hpspmm_debug_grouped_waits changes it, and withholds the copies.
+constexpr int64_t kWaitLimit = 4000000000ll;
+std::atomic<int64_t> g_wait_limit{kWaitLimit};
+std::atomic<int> g_withhold{0};
 
 typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -870,6 +899,13 @@ bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
+extern "C" int hpspmm_debug_grouped_waits(int64_t cycles, int32_t withhold) {
+  if (cycles < 0) return HPSPMM_ERR_INVALID;
+  g_wait_limit.store(cycles > 0 ? cycles : kWaitLimit, std::memory_order_relaxed);
+  g_withhold.store(withhold != 0, std::memory_order_relaxed);
+  return HPSPMM_OK;
+}
+
 int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type, const void* X, int64_t ldx,
                                   const void* W, bool out_first, const int32_t* offsets, void* Y, cudaStream_t s) {
   const bool half = type == HPSPMM_TYPE_F16;
@@ -887,7 +923,8 @@ int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t
   for (int64_t g0 = 0; g0 < G; g0 += kMaxGroups) {
     const int64_t gn = std::min<int64_t>(kMaxGroups, G - g0);
     c.a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, {(int)R, 0}, nullptr,
-           ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS, W, X, wsize[0], ldx};
+           ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS, W, X, wsize[0], ldx,
+           g_wait_limit.load(std::memory_order_relaxed), g_withhold.load(std::memory_order_relaxed)};
     c.units = (std::min(R, gn) + R / c.tile.rows) * across;
     HPSPMM_CUDA_TRY(ctx, half ? launch_product<__half>(ctx, c, out_first, s) : launch_product<__nv_bfloat16>(ctx, c, out_first, s));
   }
@@ -908,7 +945,7 @@ int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int
   const int64_t units = (G + p.slots) * ((I + c.rows - 1) / c.rows) * ((J + kLanes - 1) / kLanes);
   if (units > kMaxTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
   const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, p, slots, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS,
-                         B, A, ldb, lda};
+                         B, A, ldb, lda, g_wait_limit.load(std::memory_order_relaxed), g_withhold.load(std::memory_order_relaxed)};
   cudaError_t e;
   if (half)
     e = tma ? launch_weight_grad<__half, true>(ctx, a, ma, mb, dW, c, units, s) : launch_weight_grad<__half, false>(ctx, a, ma, mb, dW, c, units, s);

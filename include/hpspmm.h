@@ -584,6 +584,11 @@ HPSPMM_API double hpspmm_sddmm_algorithmic_bytes(int64_t M_ref, int64_t N_ref, i
  * (spmm/starml/basic/allocator_cuda.cpp:5-13). */
 HPSPMM_API int hpspmm_debug_fail_device_alloc(int64_t nth, int64_t count);
 
+/* Test seam: how long (in cycles of an SM) a wait inside the tensor-core kernels of the grouped products may take from the
+ * next call on (0: the default, about two seconds), and whether those kernels leave their copies out (withhold), so that
+ * the waits for them run out: such a call writes nothing of use and counts in hpspmm_ctx_timeouts.  Process-wide. */
+HPSPMM_API int hpspmm_debug_grouped_waits(int64_t cycles, int32_t withhold);
+
 /* ---- diagnostics: load-path ceilings ---------------------------------------------------------------
  * Times the gather shape of the product kernels alone (lane groups of row_bytes / 16 lanes,
  * one 16-byte load per lane, four gathers in flight per lane, no sparse stream, no stores):

@@ -406,3 +406,48 @@ def test_beside_the_librarys_products(ops):
     assert ref.outside(y, want, tol) == 0 and ref.outside(dw, want_w, tol_w) == 0 and ops.timeouts() == 0
     want, tol = ref.grouped(X[:8], W, off // 400)
     assert ref.outside(few, want, tol) == 0
+
+
+# One call of each kind of kernel: (rows of the groups, K, N).  Pairs of blocks, 256 rows to a tile, 128, 64, clusters of two to
+# eight blocks, widths that no copy engine takes; the gradients come with each of them.
+KINDS = [([4000, 0, 3000, 33], 256, 1024), ([6000, 0, 7001, 500], 72, 384), ([600], 1024, 1024), ([300, 9], 256, 136), ([40], 1024, 2048),
+         ([16], 2048, 1024), ([3, 5], 4096, 256), ([300, 40], 333, 131), ([3], 1001, 24), ([20_000], 64, 40)]
+
+
+@pytest.fixture
+def waits(pkg):
+    f = pkg.load_library().hpspmm_debug_grouped_waits
+    yield f
+    f(0, 0)
+
+
+@pytest.mark.parametrize("sizes,K,N", KINDS)
+def test_a_wait_that_runs_out_ends_the_call(pkg, waits, sizes, K, N):
+    """Copies that never come: every block gives up, all of its warps together, and the next calls are as ever."""
+    gen = torch.Generator("cuda").manual_seed(K)
+    R, G = sum(sizes), len(sizes)
+    X, dY = (torch.randn((R, c), device="cuda", generator=gen).bfloat16() for c in (K, N))
+    W, off = _weights(G, K, N, torch.bfloat16, gen, False), _offsets(sizes)
+    Y, dW = torch.empty((R, N), dtype=X.dtype, device="cuda"), torch.empty_like(W)
+    need = pkg.load_library().hpspmm_grouped_weight_grad_workspace(R, G, K, N, pkg.TYPE_BF16, 0)
+    space = torch.empty(max(need, 256), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def product(ctx):
+        ctx.grouped_product(R, G, K, N, pkg.TYPE_BF16, X.data_ptr(), K, W.data_ptr(), 0, off.data_ptr(), Y.data_ptr(), stream)
+
+    def gradient(ctx):
+        ctx.grouped_weight_grad(R, G, K, N, pkg.TYPE_BF16, X.data_ptr(), K, dY.data_ptr(), N, off.data_ptr(), dW.data_ptr(), 0, space.data_ptr(),
+                                need, stream)
+
+    for call, out, (want, tol) in ((product, Y, ref.grouped(X, W, off)), (gradient, dW, ref.grouped_weight(X, dY, off))):
+        with pkg.Context(0) as ctx:
+            assert waits(200_000, 1) == pkg.OK
+            call(ctx)
+            assert ctx.timeouts() > 0
+            assert waits(0, 0) == pkg.OK
+            seen = ctx.timeouts()
+            for _ in range(3):
+                call(ctx)
+            assert ref.outside(out, want, tol) == 0 and ctx.timeouts() == seen
