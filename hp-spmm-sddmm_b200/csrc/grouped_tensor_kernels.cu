@@ -50,7 +50,7 @@ struct tensor_args {
   // the operands on the lanes and on the N side, for calls whose tiles TMA cannot fetch: rows ld elements apart
   const void *a, *b;
   int64_t lda, ldb;
-  long long wait_limit;   // cycles
+  long long wait_limit;   // cycles, see wait_state
   int withhold;           // (for tests) nothing is copied, so that the waits for the copies run out
 };
 
@@ -91,8 +91,10 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 // What the waits of a block share.
 struct wait_state {
   int failed;          // one of them has been given up, so all others are
-  long long limit;     // cycles that one may take
+  long long limit;     // cycles that one may take beside kStageLimit for every stage that comes in meanwhile
 };
+// A stage takes 0.3 us with TMA and 2.1 at most without (4,200 cycles); a tile has up to 2^21 of them.
+constexpr long long kStageLimit = 20000;
 // By one thread.  Whoever gives up says so in `failed`, and all others give up with it.
 __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile wait_state* w) {
   const long long begin = clock64();
@@ -109,21 +111,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return mbar_try<false>(bar, parity) || mbar_wait_slow(bar, parity, w);
 }
 // By a whole warp, with the same answer in all lanes: what follows are instructions that all of them have to reach, so that
-// lanes which gave up while others did not would leave those waiting for good.
+// lanes which gave up while others did not would leave those waiting for good.  stages: how many may come in before the wait
+// is over; a tile's for its accumulator.
 template <bool CLUSTER>
-__device__ __noinline__ bool mbar_wait_warp_slow(uint32_t bar, uint32_t parity, volatile wait_state* w) {
+__device__ __noinline__ bool mbar_wait_warp_slow(uint32_t bar, uint32_t parity, volatile wait_state* w, int stages) {
   const long long begin = clock64();
   while (true) {
     if (__all_sync(0xffffffffu, mbar_try<CLUSTER>(bar, parity))) return true;
-    if (__any_sync(0xffffffffu, w->failed || clock64() - begin > w->limit)) {
+    if (__any_sync(0xffffffffu, w->failed || clock64() - begin > w->limit + stages * kStageLimit)) {
       w->failed = 1;
       return false;
     }
   }
 }
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile wait_state* w) {
-  return __all_sync(0xffffffffu, mbar_try<CLUSTER>(bar, parity)) || mbar_wait_warp_slow<CLUSTER>(bar, parity, w);
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile wait_state* w, int stages = 0) {
+  return __all_sync(0xffffffffu, mbar_try<CLUSTER>(bar, parity)) || mbar_wait_warp_slow<CLUSTER>(bar, parity, w, stages);
 }
 
 // PAIR: the barrier may be the one of the pair's other block (`bar` is an address in the cluster's window)
@@ -568,12 +571,15 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   } else if (kWeight && TMA && warp == 3) {   // the rows behind a group, up to the end of the instruction's depth, become zeros
     int s = 0;
     uint32_t phase = 0;   // a bit for each stage
+    int stages = 0;       // since the last one that was cut short
     for (int u = first; u < units; u += step) {
       const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
       if (t.stages == 0) continue;
       s = (s + t.stages - 1) % STAGES;
+      stages = min(stages + t.stages, 1 << 30);
       if (cut_short(t, t.stages - 1)) {
-        if (!mbar_wait_warp(cut_full(s), phase >> s & 1, &waits)) break;
+        if (!mbar_wait_warp(cut_full(s), phase >> s & 1, &waits, stages)) break;
+        stages = 0;
         phase ^= 1u << s;
         const uint32_t src = base + s * kStage;
         const int left = t.end - t.begin - (t.stages - 1) * kDepth;
@@ -636,7 +642,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
     if (CL > 1) cluster_wait();
     for (int u = first; u < units; u += step) {
       const tile t = tile_at<MODE, BN, CL, PAIR>(a, ends, slot_ends, u, rank);
-      if (!mbar_wait_warp(acc_full(acc), acc_phase, &waits)) break;
+      if (!mbar_wait_warp(acc_full(acc), acc_phase, &waits, t.stages)) break;
       tensor_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(q * 32) << 16);
       const int col = t.col0 + q * 32 + lane;
@@ -676,7 +682,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
       } else {
         // Every block takes 1 / CL of the tile's rows and gets the others' parts of them pushed into its shared memory.
         const int share = (t.rows + 15) / 16 * 16 / CL;
-        if (!mbar_wait_warp<true>(parts_empty, part_phase ^ 1, &waits)) break;
+        if (!mbar_wait_warp<true>(parts_empty, part_phase ^ 1, &waits, t.stages)) break;
         const uint32_t mine = smem_of(parts + rank * share * kLanes + q * 32 + lane);
         int to_rank = 0, r = 0;
         uint32_t at = in_block(mine, 0);
@@ -702,7 +708,7 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
           for (int p = 0; p < CL; ++p) mbar_arrive_remote(parts_full, p);
         }
         __syncwarp();
-        if (!mbar_wait_warp<true>(parts_full, part_phase, &waits)) break;
+        if (!mbar_wait_warp<true>(parts_full, part_phase, &waits, t.stages)) break;
         for (int r = 0; r < share; ++r) {
           float sum = 0.f;
 #pragma unroll
@@ -751,7 +757,8 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
-// Of a wait, in cycles: about two seconds.  hpspmm_debug_grouped_waits changes it, and withholds the copies.
+// Of a wait, in cycles: about two seconds (and kStageLimit for a stage).  hpspmm_debug_grouped_waits changes it, and withholds
+// the copies.
 constexpr int64_t kWaitLimit = 4000000000ll;
 std::atomic<int64_t> g_wait_limit{kWaitLimit};
 std::atomic<int> g_withhold{0};

@@ -584,9 +584,10 @@ HPSPMM_API double hpspmm_sddmm_algorithmic_bytes(int64_t M_ref, int64_t N_ref, i
  * (spmm/starml/basic/allocator_cuda.cpp:5-13). */
 HPSPMM_API int hpspmm_debug_fail_device_alloc(int64_t nth, int64_t count);
 
-/* Test seam: how long (in cycles of an SM) a wait inside the tensor-core kernels of the grouped products may take from the
- * next call on (0: the default, about two seconds), and whether those kernels leave their copies out (withhold), so that
- * the waits for them run out: such a call writes nothing of use and counts in hpspmm_ctx_timeouts.  Process-wide. */
+/* Test seam: how long (in cycles of an SM) a wait inside the tensor-core kernels of the grouped products may take, beside
+ * what it is allowed for the operands that come in meanwhile, from the next call on (0: the default, about two seconds), and
+ * whether those kernels leave their copies out (withhold), so that the waits for them run out: such a call writes nothing
+ * of use and counts in hpspmm_ctx_timeouts.  Process-wide. */
 HPSPMM_API int hpspmm_debug_grouped_waits(int64_t cycles, int32_t withhold);
 
 /* ---- diagnostics: load-path ceilings ---------------------------------------------------------------
@@ -610,8 +611,8 @@ HPSPMM_API int hpspmm_probe_gather_gbs(hpspmm_ctx* ctx, int32_t row_bytes, int64
 HPSPMM_API int hpspmm_ctx_tma_fallbacks(hpspmm_ctx* ctx, int64_t* count);
 
 /* Number of blocks of the tensor-core kernels of the grouped products, since the context was created, that gave up a wait
- * inside the kernel after about two seconds (expected: 0).  The outputs of such a call are not to be used.
- * Synchronises the device. */
+ * inside the kernel: after about two seconds, and 10 us more for every 64 of the depth that come in meanwhile (expected: 0).
+ * The outputs of such a call are not to be used.  Synchronises the device. */
 HPSPMM_API int hpspmm_ctx_timeouts(hpspmm_ctx* ctx, int64_t* count);
 
 /* The same random rows through the tensor memory accelerator: producer warps fetch four rows per

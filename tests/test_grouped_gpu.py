@@ -451,3 +451,29 @@ def test_a_wait_that_runs_out_ends_the_call(pkg, waits, sizes, K, N):
             for _ in range(3):
                 call(ctx)
             assert ref.outside(out, want, tol) == 0 and ctx.timeouts() == seen
+
+
+@pytest.mark.parametrize("case", ["lines", "neighbour", "deep lines", "deep"])
+def test_a_wait_lasts_as_long_as_its_tile(pkg, waits, case):
+    """Tiles of several milliseconds under a limit of 50 microseconds, which comes on top of the time that a tile's stages may
+    take.  Gradients of one long group among many (which is not cut into pieces) at a width that no copy engine takes;
+    one behind which the same block has a group that ends inside an instruction's depth; products over a long depth."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    with pkg.Context(0) as ctx:
+        assert waits(100_000, 0) == pkg.OK
+        if case.startswith("deep"):
+            R, K, N = 8, (1 << 20) + 1 if case == "deep lines" else 1 << 23, 8
+            X, W, off = torch.randn((R, K), device="cuda", generator=gen).bfloat16(), _weights(1, K, N, torch.bfloat16, gen, False), _offsets([R])
+            out, (want, tol) = torch.full((R, N), float("nan"), dtype=X.dtype, device="cuda"), ref.grouped(X, W, off)
+            torch.cuda.synchronize()
+            ctx.grouped_product(R, 1, K, N, pkg.TYPE_BF16, X.data_ptr(), K, W.data_ptr(), 0, off.data_ptr(), out.data_ptr())
+        else:
+            width = 3 if case == "lines" else 64
+            sizes = [0] * 2100
+            sizes[0], sizes[torch.cuda.get_device_properties(0).multi_processor_count] = 1 << 20, 5
+            R, G, off = sum(sizes), len(sizes), _offsets(sizes)
+            X, dY = (torch.randn((R, width), device="cuda", generator=gen).bfloat16() for _ in range(2))
+            out, (want, tol) = torch.full((G, width, width), float("nan"), dtype=X.dtype, device="cuda"), ref.grouped_weight(X, dY, off)
+            torch.cuda.synchronize()
+            ctx.grouped_weight_grad(R, G, width, width, pkg.TYPE_BF16, X.data_ptr(), width, dY.data_ptr(), width, off.data_ptr(), out.data_ptr(), 0)
+        assert ctx.timeouts() == 0 and ref.outside(out, want, tol) == 0
