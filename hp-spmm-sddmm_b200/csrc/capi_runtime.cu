@@ -75,6 +75,16 @@ int hpspmm_ctx_create(int device_ordinal, hpspmm_ctx** out) {
     return e == cudaErrorMemoryAllocation ? HPSPMM_ERR_OOM : HPSPMM_ERR_CUDA;
   }
   cudaMemset(ctx->flag, 0, 256);
+  e = cudaHostAlloc((void**)&ctx->alarm, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+  if (e == cudaSuccess) e = cudaHostGetDevicePointer((void**)&ctx->alarm_dev, ctx->alarm, 0);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    if (ctx->alarm) cudaFreeHost(ctx->alarm);
+    cudaFree(ctx->flag);
+    delete ctx;
+    return e == cudaErrorMemoryAllocation ? HPSPMM_ERR_OOM : HPSPMM_ERR_CUDA;
+  }
+  *ctx->alarm = 0;
   *out = ctx;
   return HPSPMM_OK;
 }
@@ -87,6 +97,7 @@ int hpspmm_ctx_destroy(hpspmm_ctx* ctx) {
   if (ctx->counters) cudaFree(ctx->counters);
   if (ctx->stage) cudaFree(ctx->stage);
   if (ctx->flag) cudaFree(ctx->flag);
+  if (ctx->alarm) cudaFreeHost(ctx->alarm);
   for (int i = 0; i < 3; ++i)
     if (ctx->pipe_streams[i]) cudaStreamDestroy(ctx->pipe_streams[i]);
   for (int i = 0; i < 8; ++i)

@@ -363,7 +363,7 @@ int check_distill(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int32_t type
   HPSPMM_REQUIRE(ctx, tau >= 1.17549435e-38f && tau <= 3.402823466e38f, "the temperature must be positive, normal and finite");
   if (T > 2147483646ll || V > 2147483646ll) return hpspmm_unsupported(ctx, "more than 2^31 - 2 rows or columns");
   if (k > kMaxEntries) return hpspmm_unsupported(ctx, "more than 1024 entries of the teacher for a row");
-  return HPSPMM_OK;
+  return hpspmm_report_timeout(ctx);
 }
 
 }  // namespace

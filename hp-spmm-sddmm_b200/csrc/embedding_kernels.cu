@@ -578,7 +578,7 @@ int check_embedding(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, int32_t ty
   HPSPMM_REQUIRE(ctx, ld >= 0, "negative row stride");
   if (T > 2147483646ll || N > 2147483646ll || K > 2147483646ll)
     return hpspmm_unsupported(ctx, "more than 2^31 - 2 positions, rows or columns");
-  return HPSPMM_OK;
+  return hpspmm_report_timeout(ctx);
 }
 
 }  // namespace

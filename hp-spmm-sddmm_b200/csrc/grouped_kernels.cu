@@ -374,7 +374,7 @@ int check_grouped(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, i
   HPSPMM_REQUIRE(ctx, hpspmm::dense_type_size(type) != 0, "unknown element type");
   if (R > 2147483646ll || G > 1048576 || K > 2147483646ll || N > 2147483646ll)
     return hpspmm_unsupported(ctx, "more than 2^31 - 2 rows or columns, or 2^20 groups");
-  return HPSPMM_OK;
+  return ctx ? hpspmm_report_timeout(ctx) : HPSPMM_OK;
 }
 
 }  // namespace

@@ -46,7 +46,7 @@ struct tensor_args {
   int zero_rows;       // products: whether this launch clears the rows of no group
   piece_plan plan;     // gradients
   float* slots;
-  int* timeouts;
+  int *timeouts, *alarm;   // counted and told where a wait was given up
   // the operands on the lanes and on the N side, for calls whose tiles TMA cannot fetch: rows ld elements apart
   const void *a, *b;
   int64_t lda, ldb;
@@ -738,7 +738,11 @@ grouped_tensor_kernel(const tensor_args a, const __grid_constant__ CUtensorMap m
   tensor_fence_before();
   __syncthreads();
   if (waits.failed) {   // what was started lands before the memory is given back
-    if (threadIdx.x == 0) atomicAdd(a.timeouts, 1);
+    if (threadIdx.x == 0) {
+      atomicAdd(a.timeouts, 1);
+      *static_cast<volatile int*>(a.alarm) = 1;
+      __threadfence_system();
+    }
     const long long begin = clock64();
     while (clock64() - begin < 4000000ll) __nanosleep(1000);
     __syncwarp();
@@ -930,7 +934,7 @@ int hpspmm_grouped_product_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t
   for (int64_t g0 = 0; g0 < G; g0 += kMaxGroups) {
     const int64_t gn = std::min<int64_t>(kMaxGroups, G - g0);
     c.a = {offsets, (int)R, (int)G, (int)g0, (int)gn, (int)K, 0, (int)N, g0 == 0, {(int)R, 0}, nullptr,
-           ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS, W, X, wsize[0], ldx,
+           ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS, ctx->alarm_dev, W, X, wsize[0], ldx,
            g_wait_limit.load(std::memory_order_relaxed), g_withhold.load(std::memory_order_relaxed)};
     c.units = (std::min(R, gn) + R / c.tile.rows) * across;
     HPSPMM_CUDA_TRY(ctx, half ? launch_product<__half>(ctx, c, out_first, s) : launch_product<__nv_bfloat16>(ctx, c, out_first, s));
@@ -952,7 +956,7 @@ int hpspmm_grouped_weight_grad_tensor(hpspmm_ctx* ctx, int64_t R, int64_t G, int
   const int64_t units = (G + p.slots) * ((I + c.rows - 1) / c.rows) * ((J + kLanes - 1) / kLanes);
   if (units > kMaxTiles) return hpspmm_unsupported(ctx, "more than 2^31 tiles");
   const tensor_args a = {offsets, (int)R, (int)G, 0, (int)G, 0, (int)I, (int)J, 0, p, slots, ctx->flag + HPSPMM_FLAG_TENSOR_TIMEOUTS,
-                         B, A, ldb, lda, g_wait_limit.load(std::memory_order_relaxed), g_withhold.load(std::memory_order_relaxed)};
+                         ctx->alarm_dev, B, A, ldb, lda, g_wait_limit.load(std::memory_order_relaxed), g_withhold.load(std::memory_order_relaxed)};
   cudaError_t e;
   if (half)
     e = tma ? launch_weight_grad<__half, true>(ctx, a, ma, mb, dW, c, units, s) : launch_weight_grad<__half, false>(ctx, a, ma, mb, dW, c, units, s);

@@ -34,6 +34,8 @@ struct hpspmm_ctx {
   // streams of the host-buffer entry point: uploads, kernels, downloads (created on first use)
   cudaStream_t pipe_streams[3];
   cudaEvent_t pipe_events[8];   // "A has landed" and, per buffer, slab uploaded / multiplied / downloaded
+  int* alarm;      // a word of mapped host memory: kernels set it where a wait was given up (hpspmm_report_timeout)
+  int* alarm_dev;  // the same for the device
   char err[256];
 };
 
@@ -182,6 +184,14 @@ static inline int hpspmm_set_err(hpspmm_ctx* ctx, int status, const char* what, 
 static inline int hpspmm_unsupported(hpspmm_ctx* ctx, const char* what) {
   if (ctx) snprintf(ctx->err, sizeof(ctx->err), "unsupported: %s", what);
   return HPSPMM_ERR_UNSUPPORTED;
+}
+
+// Whether a product by group whose wait ran out has finished since the last question, as the status of the call that asks.
+// The host reads a word of its own memory: no synchronisation.
+static inline int hpspmm_report_timeout(hpspmm_ctx* ctx) {
+  if (__atomic_load_n(ctx->alarm, __ATOMIC_RELAXED) == 0 || __atomic_exchange_n(ctx->alarm, 0, __ATOMIC_RELAXED) == 0) return HPSPMM_OK;
+  snprintf(ctx->err, sizeof(ctx->err), "an earlier product by group gave up a wait: its outputs are not to be used; nothing was done now");
+  return HPSPMM_ERR_TIMEOUT;
 }
 
 // Makes the context's device current for the calling thread for the duration of a call.

@@ -172,7 +172,9 @@ def grouped_product(X, W, offsets):
     ascending int32 on the GPU.  Rows of no group (behind the last one of a padded batch) become zeros.
 
     W may be the transpose of a contiguous [G, N, K] (``W.transpose(1, 2)`` of the weights of linear layers): it is
-    read as it lies, and its gradient lies the same way.  float32, float16 or bfloat16, all of one type."""
+    read as it lies, and its gradient lies the same way.  float32, float16 or bfloat16, all of one type.
+
+    Waits inside the 16-bit kernels are bounded; one that runs out spoils its call, which a later call reports (``timeouts``)."""
     if _plain(X, W, offsets):
         return _C.grouped_product(X, W, offsets)
     return torch.ops.hpspmm.grouped_product.default(X, W, offsets)
@@ -191,6 +193,7 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0):
 
 def timeouts(device=None):
     """How many blocks of the grouped products' tensor-core kernels have given up a wait on this GPU (expected 0; what
-    such a call wrote is not to be used).  Waits for the device."""
+    such a call wrote is not to be used).  Waits for the device.  The first call of these operators that finds such a product
+    done raises an error by itself; after a last step, or replays of a graph, ask here."""
     index = None if device is None else torch.device(device).index
     return _C.timeouts(torch.cuda.current_device() if index is None else index)

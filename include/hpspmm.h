@@ -325,7 +325,7 @@ HPSPMM_API int hpspmm_layer_update_values(hpspmm_ctx* ctx, hpspmm_layer* layer,
  * (rows of a table by id), one block to a group of rows (a matrix for each relation type or expert), a few samples to a
  * row (a teacher's largest logits).  Element types below; sums are kept in 32 bits and rounded once.  Rows of the
  * operands that are read may lie `ld` elements apart, what is written is contiguous.  All of them only enqueue
- * kernels: no allocation, no synchronisation, no state between calls, so they can be captured into a CUDA graph, and
+ * kernels: no allocation, no synchronisation, no state between calls (but hpspmm_ctx_timeouts), so they can be captured into a CUDA graph, and
  * calls that share a context may overlap on the GPU (not on the host: one call on a context at a time).  The
  * reference has no counterpart. */
 enum { HPSPMM_TYPE_F32 = 0, HPSPMM_TYPE_F16 = 1, HPSPMM_TYPE_BF16 = 2 };
@@ -612,7 +612,10 @@ HPSPMM_API int hpspmm_ctx_tma_fallbacks(hpspmm_ctx* ctx, int64_t* count);
 
 /* Number of blocks of the tensor-core kernels of the grouped products, since the context was created, that gave up a wait
  * inside the kernel: after about two seconds, and 10 us more for every 64 of the depth that come in meanwhile (expected: 0).
- * The outputs of such a call are not to be used.  Synchronises the device. */
+ * The outputs of such a call are not to be used.  Synchronises the device.  The first of the dense
+ * operators by index (hpspmm_embedding_*, hpspmm_grouped_*, hpspmm_topk_distill_*) on the context that finds such a kernel done
+ * returns HPSPMM_ERR_TIMEOUT without doing anything; it waits for nothing to find out, so it may be a later one than the
+ * next, and a graph's replays are seen by calls outside it. */
 HPSPMM_API int hpspmm_ctx_timeouts(hpspmm_ctx* ctx, int64_t* count);
 
 /* The same random rows through the tensor memory accelerator: producer warps fetch four rows per

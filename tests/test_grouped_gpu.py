@@ -448,6 +448,9 @@ def test_a_wait_that_runs_out_ends_the_call(pkg, waits, sizes, K, N):
             assert ctx.timeouts() > 0
             assert waits(0, 0) == pkg.OK
             seen = ctx.timeouts()
+            with pytest.raises(pkg.HpspmmError, match="gave up") as e:      # told once, by the next call
+                call(ctx)
+            assert e.value.status == pkg.ERR_TIMEOUT
             for _ in range(3):
                 call(ctx)
             assert ref.outside(out, want, tol) == 0 and ctx.timeouts() == seen
@@ -477,3 +480,78 @@ def test_a_wait_lasts_as_long_as_its_tile(pkg, waits, case):
             torch.cuda.synchronize()
             ctx.grouped_weight_grad(R, G, width, width, pkg.TYPE_BF16, X.data_ptr(), width, dY.data_ptr(), width, off.data_ptr(), out.data_ptr(), 0)
         assert ctx.timeouts() == 0 and ref.outside(out, want, tol) == 0
+
+
+def test_whoever_calls_next_is_told_of_a_wait_that_ran_out(pkg, waits):
+    """Every dense operator of the context, once, and with nothing done; refused arguments are refused as ever."""
+    bf16 = torch.bfloat16
+    X, W, off, Y = (torch.ones(s, dtype=bf16, device="cuda") for s in ((40, 64), (1, 64, 8), (1,), (40, 8)))
+    off = _offsets([40])
+    ids, z, teacher = torch.zeros(40, dtype=torch.int64, device="cuda"), torch.zeros((40, 8), device="cuda"), torch.zeros(40, device="cuda")
+    loss, stats, out = (torch.full(s, 5.0, device="cuda") for s in ((40,), (40, 2), (40, 8)))
+    space = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    p = [t.data_ptr() for t in (X, W, off, Y, ids, z, teacher, loss, stats, out, space)]
+    x, w, o, y, i, zz, te, lo, st, ou, sp = p
+    with pkg.Context(0) as ctx:
+        def product(rows=40):
+            ctx.grouped_product(rows, 1, 64, 8, pkg.TYPE_BF16, x, 64, w, 0, o, y)
+        for call in (lambda: ctx.embedding_forward(40, 40, 8, pkg.TYPE_F32, i, 8, zz, 8, 1.0, ou),
+                     lambda: ctx.embedding_backward(40, 40, 8, pkg.TYPE_F32, i, 8, zz, 8, 1.0, ou, sp, 1 << 20), product,
+                     lambda: ctx.grouped_weight_grad(40, 1, 64, 8, pkg.TYPE_BF16, x, 64, y, 8, o, w, 0),
+                     lambda: ctx.topk_distill_forward(40, 8, 1, pkg.TYPE_F32, zz, 8, i, 8, te, 1.0, lo, st),
+                     lambda: ctx.topk_distill_backward(40, 8, 1, pkg.TYPE_F32, zz, 8, i, 8, te, 1.0, st, te, 1, ou)):
+            waits(100_000, 1)
+            product()
+            waits(0, 0)
+            torch.cuda.synchronize()
+            before = [t.clone() for t in (loss, stats, out, W)]
+            with pytest.raises(pkg.HpspmmError) as e:
+                product(-1)
+            assert e.value.status == pkg.ERR_INVALID
+            with pytest.raises(pkg.HpspmmError, match="gave up") as e:
+                call()
+            assert e.value.status == pkg.ERR_TIMEOUT
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(before, (loss, stats, out, W)))
+            call()
+            product()
+            torch.cuda.synchronize()
+            assert bool((Y == 64 * W[0, 0, 0]).all())
+
+
+def test_pytorch_raises_after_a_wait_that_ran_out():
+    """A process of its own, whose contexts may count: a graph's replay gives up, the next call outside raises, those behind work."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+import __graft_entry__
+import dense_reference as ref
+pkg = __graft_entry__.load_package()
+ops = ref.ops_of(pkg)
+waits = pkg.load_library().hpspmm_debug_grouped_waits
+X, W, off = torch.ones((40, 64), device="cuda").half(), torch.ones((1, 64, 8), device="cuda").half(), torch.tensor([0, 40], dtype=torch.int32, device="cuda")
+ops.grouped_product(X, W, off)
+g = torch.cuda.CUDAGraph()
+waits(100_000, 1)
+with torch.cuda.graph(g):
+    ops.grouped_product(X, W, off)
+waits(0, 0)
+assert ops.timeouts() == 0
+g.replay()
+torch.cuda.synchronize()
+try:
+    ops.embedding(torch.zeros(3, dtype=torch.int64, device="cuda"), X)
+except RuntimeError as e:
+    assert "gave up" in str(e) and "status 4" in str(e), e
+else:
+    assert False
+assert bool((ops.grouped_product(X, W, off) == 64).all()) and ops.timeouts() > 0
+print("well")
+""" % (root, os.path.join(root, "tests"))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip().endswith("well"), out.stdout[-2000:]
