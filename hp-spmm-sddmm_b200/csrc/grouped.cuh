@@ -29,9 +29,10 @@ __device__ __forceinline__ void part_bounds(const int* offsets, int G, int R, in
 struct piece_plan {
   int length, slots;
 };
+constexpr int64_t kMostRows = 2147483647 - 1025;   // and columns: what the kernels add to fill a last tile stays below 2^31
 constexpr int64_t kMostDepth = 1 << 27;   // of one tile on the tensor cores: 0.6 s with TMA, 2 to 4.4 s without
 constexpr int kMostSplitGroups = 2048;   // calls of more groups are not split: they have tiles enough
-__host__ __device__ __forceinline__ int pieces_of(int rows, int length) { return rows > length ? (rows + length - 1) / length : 1; }
+__host__ __device__ __forceinline__ int pieces_of(int rows, int length) { return rows > length ? (rows - 1) / length + 1 : 1; }
 
 // Room for the pieces of all groups that have more than one: fewer than 2 R / length.
 static inline int64_t piece_slots(int64_t R, int64_t length) { return length >= R ? 0 : 2 * R / length + 1; }

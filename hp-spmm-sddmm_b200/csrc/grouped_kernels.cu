@@ -372,8 +372,8 @@ piece_plan plan_pieces(int64_t R, int64_t G, int64_t I, int64_t J, int32_t type)
 int check_grouped(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, int32_t type) {
   HPSPMM_REQUIRE(ctx, R >= 0 && G >= 0 && K >= 0 && N >= 0, "negative size");
   HPSPMM_REQUIRE(ctx, hpspmm::dense_type_size(type) != 0, "unknown element type");
-  if (R > 2147483646ll || G > 1048576 || K > 2147483646ll || N > 2147483646ll)
-    return hpspmm_unsupported(ctx, "more than 2^31 - 2 rows or columns, or 2^20 groups");
+  if (R > kMostRows || G > 1048576 || K > kMostRows || N > kMostRows)
+    return hpspmm_unsupported(ctx, "more than 2^31 - 1026 rows or columns, or 2^20 groups");
   return ctx ? hpspmm_report_timeout(ctx) : HPSPMM_OK;
 }
 

@@ -269,7 +269,7 @@ __device__ __forceinline__ tile tile_at(const tensor_args& a, const int* ends, c
       const int piece = q - (lo ? ends[lo - 1] : 0);
       if (pieces_of(max(t.end - t.begin, 0), a.plan.length) > 1) t.slot = (lo ? slot_ends[lo - 1] : 0) + piece;
       t.begin += piece * a.plan.length;
-      t.end = min(t.end, t.begin + a.plan.length);
+      t.end = t.begin + min(t.end - t.begin, a.plan.length);
     }
     t.stages = (max(t.end - t.begin, 0) + kDepth - 1) / kDepth;
     return t;
@@ -279,7 +279,7 @@ __device__ __forceinline__ tile tile_at(const tensor_args& a, const int* ends, c
   part_bounds(a.offsets, a.G, a.R, t.g, begin, end);
   // equal tiles, in steps of the instruction's 16; never more than BN rows, and as tiles = ceil(rows / BN), none is empty
   // (offsets that do not ascend can have more rows than there are, and their count of tiles is cut off)
-  const int step = min(((end - begin + tiles - 1) / tiles + 15) / 16 * 16, BN);
+  const int step = min(((end - begin - 1) / tiles + 16) / 16 * 16, BN);
   t.row0 = begin + (q - first) * step;
   t.rows = min(step, end - t.row0);
   const int stages = (a.depth + kDepth - 1) / kDepth;

@@ -150,7 +150,7 @@ Tensor grouped_weight_grad(const Tensor& X, const Tensor& dY, const Tensor& offs
   const int64_t K = x.size(1), N = dy.size(1);
   Tensor dW = transposed ? at::empty({groups, N, K}, x.options()) : at::empty({groups, K, N}, x.options());
   const int64_t bytes = hpspmm_grouped_weight_grad_workspace(x.size(0), groups, K, N, type, transposed);
-  TORCH_CHECK(bytes >= 0, "hpspmm: more than 2^31 - 2 rows or columns, or 2^20 groups");
+  TORCH_CHECK(bytes >= 0, "hpspmm: more than 2^31 - 1026 rows or columns, or 2^20 groups");
   const Tensor workspace = at::empty({bytes}, x.options().dtype(at::kByte));
   call(x.device(), "hpspmm_grouped_weight_grad", [&](hpspmm_ctx* ctx, hpspmm_stream stream) {
     return hpspmm_grouped_weight_grad(ctx, x.size(0), groups, K, N, type, x.const_data_ptr(), stride_of(x),

@@ -64,3 +64,14 @@ def test_no_block_writes_into_a_cluster_before_all_of_it_runs():
                 assert max(waits) >= 0 and max(arrives) >= 0, path
                 assert min(x for x in arrives if x >= 0) < min(x for x in waits if x >= 0), path
     assert seen == 2
+
+
+def test_sizes_whose_last_tile_would_pass_2_31(pkg):
+    """Rows and columns of the grouped products: what the kernels add to fill a tile has to stay below 2^31."""
+    need = pkg.load_library().hpspmm_grouped_weight_grad_workspace
+    most = 2 ** 31 - 1026
+    for type in (pkg.TYPE_F32, pkg.TYPE_BF16):
+        for out_first in (0, 1):
+            assert need(most, 1, 8, 8, type, out_first) > 0 and need(5, 1, most, 8, type, out_first) == 0
+            for sizes in ((most + 1, 1, 8, 8), (2 ** 31 - 2, 1, 8, 8), (5, 1, most + 1, 8), (5, 1, 8, most + 1), (5, 2 ** 20 + 1, 8, 8)):
+                assert need(*sizes, type, out_first) == -1

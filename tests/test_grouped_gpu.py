@@ -555,3 +555,40 @@ print("well")
 """ % (root, os.path.join(root, "tests"))
     out = subprocess.run([sys.executable, "-c", code], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip().endswith("well"), out.stdout[-2000:]
+
+
+def test_refusals_next_to_2_31(pkg, gpu_ctx):
+    t = torch.zeros(64, device="cuda")
+    off, at = _offsets([3]), t.data_ptr()
+    for type in (pkg.TYPE_F32, pkg.TYPE_BF16):
+        for R, K, N in ((2 ** 31 - 1025, 1, 1), (1, 2 ** 31 - 1025, 1), (1, 1, 2 ** 31 - 1025), (2 ** 31 - 2, 1, 1), (1, 1, 2 ** 31 - 2)):
+            with pytest.raises(pkg.HpspmmError) as e:
+                gpu_ctx.grouped_product(R, 1, K, N, type, at, K, at, 0, off.data_ptr(), at)
+            assert e.value.status == pkg.ERR_UNSUPPORTED
+            with pytest.raises(pkg.HpspmmError) as e:
+                gpu_ctx.grouped_weight_grad(R, 1, K, N, type, at, K, at, N, off.data_ptr(), at, 0)
+            assert e.value.status == pkg.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
+def test_nearly_2_31_rows(ops, type):
+    """One column in, one out: every row is one product, rounded once, and the gradient is a sum over pieces of 14 million rows
+    of which a few hold something."""
+    gen = torch.Generator("cuda").manual_seed(30)
+    R, dtype = 2 ** 31 - 2000, ref.TYPES[type]
+    torch.cuda.empty_cache()
+    X = torch.empty((R, 1), dtype=dtype, device="cuda").normal_(generator=gen)
+    W = torch.tensor([[[0.7]]], device="cuda").to(dtype)
+    off = torch.tensor([0, R - 3], dtype=torch.int32, device="cuda")
+    y = ops.grouped_product(X, W, off)
+    assert not y[R - 3:].any()
+    y[R - 3:] = X[R - 3:].float().mul(W[0, 0].float()).to(dtype)
+    assert all(torch.equal(b, a.float().mul(W[0, 0].float()).to(dtype)) for a, b in zip(X.split(1 << 28), y.split(1 << 28)))
+    y.zero_()
+    places = torch.tensor([0, 1 << 24, 10 ** 9, R // 2, R - 20_000_000, R - 5, R - 4], device="cuda")
+    y[places] = torch.randn((7, 1), device="cuda", generator=gen).to(dtype)
+    dw = torch.ops.hpspmm.grouped_weight_grad(X, y, off, False)
+    want, tol = ref.grouped_weight(X[places], y[places], _offsets([7]))
+    assert ref.outside(dw, want, tol) == 0
+    del X, y
+    torch.cuda.empty_cache()
