@@ -65,7 +65,8 @@ __device__ __forceinline__ bool row_any(bool v) { return NT == 32 ? __any_sync(0
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// A row of V elements at any address: `head` elements in front of the first 16-byte boundary, vectors, the rest from `tail` on.
+// A row of V elements at any address: `head` elements in front of the first 16-byte boundary, vectors, the rest from `tail` on
+// (which is counted from there: V may be so near 2^31 that a step past it would not be an int).
 template <typename T>
 struct row_parts {
   int head, vectors, tail;
@@ -140,7 +141,7 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
   if (rank == 0)
     for (int v = tid; v < at.head; v += NT) r.add(to_float(z[v]), c);
   if (rank == CL - 1)
-    for (int v = at.tail + tid; v < V; v += NT) r.add(to_float(z[v]), c);
+    for (int v = tid; v < V - at.tail; v += NT) r.add(to_float(z[at.tail + v]), c);
   const uint4* words = reinterpret_cast<const uint4*>(z + at.head);
   const int begin = (int)((int64_t)at.vectors * rank / CL), end = (int)((int64_t)at.vectors * (rank + 1) / CL);
   int v = begin + tid;
@@ -261,7 +262,7 @@ distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits
     if (slice == 0)
       for (int v = tid; v < at.head; v += NT) dz[v] = from_float<T>(value(to_float(z[v])));
     if (slice == slices - 1)
-      for (int v = at.tail + tid; v < V; v += NT) dz[v] = from_float<T>(value(to_float(z[v])));
+      for (int v = tid; v < V - at.tail; v += NT) dz[at.tail + v] = from_float<T>(value(to_float(z[at.tail + v])));
   } else {   // rows of the two that begin differently: element by element
     for (int64_t v = (int64_t)V * slice / slices + tid; v < (int64_t)V * (slice + 1) / slices; v += NT)
       dz[v] = from_float<T>(value(to_float(z[v])));

@@ -409,3 +409,32 @@ def test_few_long_rows_again_and_again_on_a_busy_gpu(ops, T):
     assert ref.outside(first[0], want, tol) == 0
     for loss, stats in held:
         assert torch.equal(loss, first[0]) and torch.equal(stats, first[1])
+
+
+@pytest.mark.parametrize("off", [0, 1])
+def test_a_row_of_nearly_2_31_columns(ops, off):
+    """All logits 0 but four: the sum over the row is known, and so is every value of the gradient."""
+    torch.cuda.empty_cache()
+    V = 2 ** 31 - 2 - off
+    z = torch.zeros(2 ** 31 - 2, dtype=torch.bfloat16, device="cuda")[off:][None]
+    ids = torch.tensor([[7, V - 1, V - 2, V]], device="cuda")                 # (the last one is no column)
+    logits = torch.tensor([4.0, 5.0, 3.0], dtype=torch.float64, device="cuda")
+    z[0, ids[0, :3]] = logits.bfloat16()
+    z[0, V // 2] = 6.0
+    teacher = torch.tensor([[1.0, 0.5, 2.0, 9.0]], device="cuda")
+    loss, stats = torch.ops.hpspmm.topk_distill(z, ids, teacher, 1.0)
+    total = float(logits.exp().sum()) + float(torch.tensor(6.0).double().exp()) + (V - 4)
+    p = torch.softmax(teacher[0, :3].double(), 0)
+    want = float((p * (p.log() - (logits - torch.tensor(total).double().log().cuda()))).sum())
+    assert abs(float(loss[0]) - want) <= 2.0 ** -18 * want
+    dz = torch.ops.hpspmm.topk_distill_backward(torch.ones(1, device="cuda"), z, ids, teacher, stats, 1.0)[0]
+    # two roundings of the exponent's parts (up to 6 of 2^-24 relative to values of up to 9), ex2, the sum, one of bf16
+    room = torch.finfo(torch.bfloat16).eps / 2 * (1 + 2.0 ** -6)
+    want = torch.cat((logits.exp() / total - p, torch.tensor([6.0], device="cuda").double().exp() / total))
+    at = torch.cat((ids[0, :3], torch.tensor([V // 2], device="cuda")))
+    assert bool(((dz[at].double() - want).abs() <= room * want.abs()).all())
+    dz[at] = float(dz[0])
+    assert abs(float(dz[0]) * total - 1) <= room
+    assert all(bool((c == dz[0]).all()) for c in dz.split(1 << 28))
+    del z, dz
+    torch.cuda.empty_cache()
