@@ -25,7 +25,8 @@ lookup_kernel(int64_t groups, int pieces, int per_row, int N, const void* ids, i
   const int64_t group = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / W;
   if (group >= groups) return;
   const int64_t t = pieces == 1 ? group : group / pieces;
-  const int first = (int)(group - t * pieces) * 4 * W + (threadIdx.x & (W - 1));
+  // (unsigned: a row may have nearly 2^31 vectors, and the last lanes step past its end)
+  const unsigned first = (unsigned)(group - t * pieces) * (4 * W) + (threadIdx.x & (W - 1)), vectors = per_row;
   const int id = load_id(ids, wide, t, N);
   const T* src = table + (int64_t)id * ld;
   T* to = out + t * ((int64_t)per_row * vec::kCount);
@@ -33,11 +34,11 @@ lookup_kernel(int64_t groups, int pieces, int per_row, int N, const void* ids, i
   if (id >= 0) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (first + u * W < per_row) v[u].raw = *reinterpret_cast<const decltype(v[u].raw)*>(src + (int64_t)(first + u * W) * vec::kCount);
+      if (first + u * W < vectors) v[u].raw = *reinterpret_cast<const decltype(v[u].raw)*>(src + (int64_t)(first + u * W) * vec::kCount);
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    if (first + u * W < per_row) {
+    if (first + u * W < vectors) {
 #pragma unroll
       for (int e = 0; e < vec::kCount; ++e) v[u].at[e] = from_float<T>(id >= 0 ? scale * to_float(v[u].at[e]) : 0.f);
       reinterpret_cast<decltype(v[u].raw)*>(to)[first + u * W] = v[u].raw;
@@ -542,7 +543,7 @@ void launch_lookup(int64_t T_, int64_t N, int64_t K, const void* ids, int wide, 
   const int per_row = (int)(K * (int64_t)sizeof(T) / BYTES);
   // rows of up to 32 (8) vectors: 8 (2) lanes with up to four each, so that as much is in flight as with wide rows
   const int W = per_row <= 8 ? 2 : (per_row <= 32 ? 8 : 32);
-  const int64_t pieces = (per_row + 4 * W - 1) / (4 * W), groups = T_ * pieces;
+  const int64_t pieces = ((int64_t)per_row + 4 * W - 1) / (4 * W), groups = T_ * pieces;
   const dim3 grid((unsigned)((groups * W + kThreads - 1) / kThreads));
   if (W == 2)
     hpspmm_launch(lookup_kernel<T, BYTES, 2>, grid, dim3(kThreads), 0, s, groups, (int)pieces, per_row, (int)N, ids, wide, (const T*)table, ld,

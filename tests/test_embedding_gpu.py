@@ -237,3 +237,15 @@ def test_one_row_of_the_gradient_for_all_positions(pkg, gpu_ctx):
     torch.cuda.synchronize()
     assert torch.equal(dtable[0], row) and not dtable[1].any() and not dtable[3].any()
     assert float((dtable[2].double() - 3 * row.double()).abs().max()) <= 3 * 2.0 ** -23 * float(row.abs().max())
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+def test_a_row_of_nearly_2_31_columns(ops, type):
+    torch.cuda.empty_cache()
+    K, gen = 2 ** 31 - 3, torch.Generator("cuda").manual_seed(31)
+    table = torch.empty((1, K), dtype=ref.TYPES[type], device="cuda").uniform_(generator=gen)
+    out = ops.embedding(torch.tensor([0, -1], device="cuda"), table, 1.5)
+    assert all(torch.equal(a.float().mul(1.5).to(table.dtype), b) for a, b in zip(table[0].split(1 << 28), out[0].split(1 << 28)))
+    assert not any(bool(c.any()) for c in out[1].split(1 << 28))
+    del table, out
+    torch.cuda.empty_cache()
