@@ -1,6 +1,6 @@
 // Loss of rows of logits against a teacher of whose logits only a few for each row are kept, and its gradient.
 //   p     = softmax over the row's entries of (teacher / tau); an entry counts when its id lies in [0, V) and its logit is
-//           above -infinity
+//           above -infinity (so not when it is NaN)
 //   loss  = tau^2 * sum_j p_j (log p_j - log softmax(z / tau)[id_j])          0 for a row without entries
 //   dz_v  = dloss * tau * (softmax(z / tau)_v - sum over j with id_j = v of p_j)      zeros for a row without entries
 // The teacher's rows are the values of a sparse matrix whose pattern samples the dense one, as in SDDMM.
@@ -133,7 +133,8 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
   if (rank == 0)
     for (int j = tid; j < k; j += NT) {   // an entry that does not count: -infinity
       const int id = load_id(ids, wide, row * k + j, V);
-      of_teacher[slot][j] = id >= 0 ? teacher[row * k + j] : -INFINITY;
+      const float t = teacher[row * k + j];
+      of_teacher[slot][j] = id >= 0 && t > -INFINITY ? t : -INFINITY;   // (not one that is no number either)
       of_student[slot][j] = id >= 0 ? to_float(z[id]) : 0.f;
     }
   const row_parts<T> at(z, V);
@@ -193,7 +194,6 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
   row_sync<NT>();
   float t_top = -INFINITY;
   for (int j = tid; j < k; j += NT) t_top = fmaxf(t_top, of_teacher[slot][j]);
-  // (no entry but one of -infinity does not count; one that is no number leaves the maximum alone)
   bool some = false;
   for (int j = tid; j < k; j += NT) some = some || of_teacher[slot][j] != -INFINITY;
   some = row_any<NT>(some);
@@ -241,7 +241,7 @@ distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits
   bool some = false;
   for (int j = tid; j < k; j += NT) {
     const float t = teacher[row * k + j];
-    const int i = t == -INFINITY ? -1 : load_id(ids, wide, row * k + j, V);
+    const int i = t > -INFINITY ? load_id(ids, wide, row * k + j, V) : -1;
     id[j] = i, p[j] = t;
     if (i >= 0) some = true, t_top = fmaxf(t_top, t);
   }

@@ -184,8 +184,8 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0):
     """``temperature**2 * KL(teacher || student)`` of every row, the teacher known by its k largest logits: logits
     [..., V], teacher_ids (int32 or int64) and teacher_logits [..., k], k up to 1024; float32 [...] comes out.
 
-    The teacher's softmax runs over the entries whose id lies in [0, V) and whose logit is above -inf; a row without
-    any has loss 0 and a gradient of zeros.  Differentiable in the logits, once."""
+    The teacher's softmax runs over the entries whose id lies in [0, V) and whose logit is above -inf (NaN is not); a
+    row without any has loss 0 and a gradient of zeros.  Differentiable in the logits, once."""
     if _plain(logits, teacher_ids, teacher_logits):
         return _C.topk_distill(logits, teacher_ids, teacher_logits, temperature)
     return torch.ops.hpspmm.topk_distill.default(logits, teacher_ids, teacher_logits, temperature)[0]

@@ -371,8 +371,8 @@ HPSPMM_API int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G,
 /* For every row z of T x V logits and the k entries (ids[j], teacher_logits[j]) its teacher kept:
  *   p    = softmax over the entries of teacher_logits / temperature
  *   loss = temperature^2 * sum_j p_j (log p_j - log softmax(z / temperature)[ids[j]])
- * An entry counts when its id lies in [0, V) and its logit is above -infinity; ids that come twice count twice.  A row
- * without entries has loss 0.  k is at most 1024 (HPSPMM_ERR_UNSUPPORTED beyond).  loss: T floats.  stats: T x 2
+ * An entry counts when its id lies in [0, V) and its logit is above -infinity (NaN is not); ids that come twice count
+ * twice.  A row without entries has loss 0.  k is at most 1024 (HPSPMM_ERR_UNSUPPORTED beyond).  loss: T floats.  stats: T x 2
  * floats for the gradient (largest logit of the row, sum of exp((z - it) / temperature)), or NULL. */
 HPSPMM_API int hpspmm_topk_distill_forward(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k, int32_t type,
                                            const void* logits, int64_t ld_logits, const void* ids,

@@ -438,3 +438,18 @@ def test_a_row_of_nearly_2_31_columns(ops, off):
     assert all(bool((c == dz[0]).all()) for c in dz.split(1 << 28))
     del z, dz
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("V,k", [(29, 6), (5000, 6), (700, 200), (40_000, 6)])
+def test_teachers_that_are_no_number_do_not_count(ops, V, k):
+    """An entry counts when its logit is above -infinity, which NaN is not, whatever its id."""
+    gen = torch.Generator("cuda").manual_seed(32)
+    for dtype in (torch.float32, torch.bfloat16):
+        z, ids, teacher = _inputs(6, V, k, dtype, gen, missing=0.0)
+        teacher[0, 0] = float("nan")
+        teacher[1, 1:] = float("nan")                 # one is left
+        teacher[2] = float("nan")                     # none is left
+        teacher[3, 1], ids[3, 2] = float("nan"), ids[3, 1]      # a column that another entry names too
+        teacher[4, :2], teacher[4, 2:4] = float("nan"), -INF
+        loss, dz = _check(ops, z, ids, teacher, 1.3)
+        assert loss[2] == 0 and not dz[2].any() and bool(torch.isfinite(loss).all()) and bool(torch.isfinite(dz).all())
