@@ -18,27 +18,32 @@ constexpr int kThreads = 256;
 
 // ---- which rows a block has ------------------------------------------------------------------------------------------
 
+// Parts that one launch of a product has.  Every block looks through them for its own, 128 at a time (so a multiple of that),
+// and with all of many in one launch the time grew with their square: 131,072 groups of 1,000 rows, 16 x 16: 118 ms, now 1.5.
+// 200,000 rows of 4,000 groups take 124 us in one launch and 123 in two.
+constexpr int kMostSearched = 33 * 128;
+
 struct row_tile {
   int g, r0, rows;   // rows [r0, r0 + rows) of part g (grouped.cuh); rows = 0: there is none
   int pieces, slot;  // gradients: pieces of the group, and where this one's goes
 };
 
-// The t-th tile of up to `length` rows, of the parts (products) or of the groups (gradients: at least one for each).  Called
-// by whole warps, each of which looks at 128 of them at a time.
+// The t-th tile of up to `length` rows, of the `parts` parts from g0 on (products) or of the groups (gradients: at least one
+// for each).  Called by whole warps, each of which looks at 128 of them at a time; kMostSearched bounds their number.
 template <bool GRADIENT>
-__device__ __forceinline__ row_tile find_row_tile(const int* offsets, int G, int R, int length, int t) {
-  const int lane = threadIdx.x & 31, parts = GRADIENT ? G : G + 2;
+__device__ __forceinline__ row_tile find_row_tile(const int* offsets, int G, int R, int length, int t, int g0, int parts) {
+  const int lane = threadIdx.x & 31;
   row_tile out = {0, 0, 0, 0, 0};
   int slots_before = 0;
   for (int base = 0; base < parts; base += 128) {
     int begin[4], end[4], tiles[4], sum = 0, slots = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part_bounds(offsets, G, R, base + lane * 4 + i, begin[i], end[i]);
+    for (int i = 0; i < 4; ++i) part_bounds(offsets, G, R, g0 + base + lane * 4 + i, begin[i], end[i]);   // (none behind G + 2)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = max(end[i] - begin[i], 0);
       if (GRADIENT)
-        tiles[i] = base + lane * 4 + i < G ? pieces_of(n, length) : 0;
+        tiles[i] = base + lane * 4 + i < parts ? pieces_of(n, length) : 0;
       else
         tiles[i] = (n + length - 1) / length;
       sum += tiles[i];
@@ -59,7 +64,7 @@ __device__ __forceinline__ row_tile find_row_tile(const int* offsets, int G, int
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (left >= 0 && left < tiles[i]) {
-            out.g = base + lane * 4 + i;
+            out.g = g0 + base + lane * 4 + i;
             out.r0 = begin[i] + left * length;
             out.rows = max(min(length, end[i] - out.r0), 0);
             out.pieces = tiles[i], out.slot = slot + left;
@@ -253,10 +258,10 @@ __device__ __forceinline__ void tile_product(const float* A, int64_t sa, const f
 template <int BN, bool OUT_FIRST, bool VEC>
 __global__ void __launch_bounds__(2 * kProductRows, BN == 64 && !OUT_FIRST ? 5 : 4)
 grouped_product_kernel(int R, int G, int K, int N, const float* __restrict__ X, int64_t ldx, const float* __restrict__ W, const int* offsets,
-                       float* __restrict__ Y, int col_tiles) {
+                       float* __restrict__ Y, int col_tiles, int g0, int parts) {
   extern __shared__ float4 tile_smem[];
   const int t = blockIdx.x / col_tiles, j0 = (blockIdx.x - t * col_tiles) * BN;
-  const row_tile w = find_row_tile<false>(offsets, G, R, kProductRows, t);
+  const row_tile w = find_row_tile<false>(offsets, G, R, kProductRows, t, g0, parts);
   if (w.rows == 0) return;
   const bool none = w.g >= G;
   const float* wg = none ? W : W + (int64_t)w.g * K * N;
@@ -276,7 +281,14 @@ grouped_weight_grad_kernel(int R, int G, int I, int J, const float* __restrict__
   t /= j_tiles;
   const int i0 = t % i_tiles * kGradientRows;
   t /= i_tiles;
-  const row_tile w = find_row_tile<true>(offsets, G, R, plan.length, t);
+  row_tile w;
+  if (plan.slots > 0) {
+    w = find_row_tile<true>(offsets, G, R, plan.length, t, 0, G);
+  } else {   // groups as they are
+    int end;
+    part_bounds(offsets, G, R, t, w.r0, end);
+    w.g = t, w.rows = max(end - w.r0, 0), w.pieces = 1;
+  }
   if (w.pieces == 0 || (w.pieces > 1 && w.slot >= plan.slots)) return;
   const float *a = A + (int64_t)w.r0 * lda + i0, *b = B + (int64_t)w.r0 * ldb + j0;
   const int rows = min(kGradientRows, I - i0), cols = min(BN, J - j0);
@@ -319,13 +331,18 @@ join_pieces_kernel(int R, int G, int64_t elements, const int* offsets, const pie
 
 // (a refused size of the shared memory shows at the launch)
 template <int BN, bool OUT_FIRST, bool VEC>
-void launch_product(int64_t R, int64_t G, int64_t K, int64_t N, const void* X, int64_t ldx, const void* W, const int32_t* offsets,
+void launch_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N, const void* X, int64_t ldx, const void* W, const int32_t* offsets,
                     void* Y, cudaStream_t s) {
   constexpr int smem = tile_shape<kProductRows, BN, true, OUT_FIRST, VEC>::kBytes;
   cudaFuncSetAttribute(grouped_product_kernel<BN, OUT_FIRST, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  const int64_t col_tiles = (N + BN - 1) / BN, blocks = ((R + kProductRows - 1) / kProductRows + G + 2) * col_tiles;
-  grouped_product_kernel<BN, OUT_FIRST, VEC><<<(unsigned)blocks, 2 * kProductRows, smem, s>>>(
-      (int)R, (int)G, (int)K, (int)N, (const float*)X, ldx, (const float*)W, offsets, (float*)Y, (int)col_tiles);
+  const int64_t col_tiles = (N + BN - 1) / BN;
+  for (int64_t g0 = 0; g0 < G + 2; g0 += kMostSearched) {
+    const int64_t parts = std::min<int64_t>(kMostSearched, G + 2 - g0);
+    const int64_t blocks = ((R + kProductRows - 1) / kProductRows + std::min(R, parts)) * col_tiles;
+    grouped_product_kernel<BN, OUT_FIRST, VEC><<<(unsigned)blocks, 2 * kProductRows, smem, s>>>(
+        (int)R, (int)G, (int)K, (int)N, (const float*)X, ldx, (const float*)W, offsets, (float*)Y, (int)col_tiles, (int)g0, (int)parts);
+    ctx->launches++;
+  }
 }
 
 template <int BN, bool VEC>
@@ -414,23 +431,22 @@ int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int
   if (type != HPSPMM_TYPE_F32 && K > kMostDepth) return hpspmm_unsupported(ctx, "16-bit products deeper than 2^27");
   if (type != HPSPMM_TYPE_F32)
     return hpspmm_grouped_product_tensor(ctx, R, G, K, N, type, X, ldx, W, w_out_first != 0, offsets, Y, s);
-  if (((R + kProductRows - 1) / kProductRows + G + 2) * ((N + 63) / 64) > 2147483647ll)
+  if (((R + kProductRows - 1) / kProductRows + std::min<int64_t>(G + 2, kMostSearched)) * ((N + 63) / 64) > 2147483647ll)
     return hpspmm_unsupported(ctx, "more than 2^31 - 1 tiles of 64 x 64");
   const bool vec = K % 4 == 0 && N % 4 == 0 && ldx % 4 == 0 && aligned16(X) && aligned16(W) && aligned16(Y);
   const bool narrow = tile_columns(N) == 64, of = w_out_first != 0;
   if (of && vec)
-    launch_product<64, true, true>(R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<64, true, true>(ctx, R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (of)
-    launch_product<64, true, false>(R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<64, true, false>(ctx, R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (vec && narrow)
-    launch_product<64, false, true>(R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<64, false, true>(ctx, R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (vec)
-    launch_product<128, false, true>(R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<128, false, true>(ctx, R, G, K, N, X, ldx, W, offsets, Y, s);
   else if (narrow)
-    launch_product<64, false, false>(R, G, K, N, X, ldx, W, offsets, Y, s);
+    launch_product<64, false, false>(ctx, R, G, K, N, X, ldx, W, offsets, Y, s);
   else
-    launch_product<128, false, false>(R, G, K, N, X, ldx, W, offsets, Y, s);
-  ctx->launches++;
+    launch_product<128, false, false>(ctx, R, G, K, N, X, ldx, W, offsets, Y, s);
   HPSPMM_CUDA_TRY(ctx, cudaGetLastError());
   return HPSPMM_OK;
 }
