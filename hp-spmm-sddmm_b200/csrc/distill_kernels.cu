@@ -114,7 +114,7 @@ struct running {
 template <typename T, int NT, int CL, int ENTRIES>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 0)
 distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
-                       const float* __restrict__ teacher, float tau, float* __restrict__ loss, float2* __restrict__ stats) {
+                       const float* __restrict__ teacher, float tau, float* __restrict__ loss, float* __restrict__ stats) {
   typedef dense_vec<T, 16> vec;
   constexpr int E = vec::kCount, kTogether = 8 / E;   // eight values to a step
   constexpr int kRows = kThreads / NT, kEntries = ENTRIES;
@@ -190,7 +190,7 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
     }
     top = most;
   }
-  if (tid == 0 && stats) stats[row] = make_float2(top, total);
+  if (tid == 0 && stats) stats[2 * row] = top, stats[2 * row + 1] = total;   // (floats: they may begin on any 4 bytes)
   row_sync<NT>();
   float t_top = -INFINITY;
   for (int j = tid; j < k; j += NT) t_top = fmaxf(t_top, of_teacher[slot][j]);
@@ -218,7 +218,7 @@ distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits,
 template <typename T, int NT, int ENTRIES>
 __global__ void __launch_bounds__(kThreads)
 distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,
-                        const float* __restrict__ teacher, float tau, const float2* __restrict__ stats,
+                        const float* __restrict__ teacher, float tau, const float* __restrict__ stats,
                         const float* __restrict__ dloss, int64_t dloss_stride, T* __restrict__ dlogits, int slices) {
   typedef dense_vec<T, 16> vec;
   constexpr int E = vec::kCount;
@@ -235,7 +235,7 @@ distill_backward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits
   int* id = id_of[slot];
   float* p = p_of[slot];
   const float c = kLog2e / tau;
-  const float2 st = stats[row];
+  const float2 st = make_float2(stats[2 * row], stats[2 * row + 1]);
   const float g = dloss[row * dloss_stride] * tau, q = 1.f / st.y;
   float t_top = -INFINITY;
   bool some = false;
@@ -324,7 +324,7 @@ cudaError_t launch_cluster(int64_t rows, int V, int k, const void* logits, int64
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3((unsigned)(rows * CL)), c.blockDim = dim3(kThreads), c.stream = s, c.attrs = &attr, c.numAttrs = CL > 1;
   return cudaLaunchKernelEx(&c, distill_forward_kernel<T, kThreads, CL, kMaxEntries>, rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, loss,
-                            (float2*)stats);
+                            stats);
 }
 
 template <typename T>
@@ -333,7 +333,7 @@ cudaError_t launch_forward(hpspmm_ctx* ctx, int64_t rows, int V, int k, const vo
   const distill_shape sh = choose_distill(ctx, rows, V, k, (int)sizeof(T));
   if (sh.warp) {
     auto* kernel = k <= kFewEntriesWarp ? distill_forward_kernel<T, 32, 1, kFewEntriesWarp> : distill_forward_kernel<T, 32, 1, kMaxEntriesWarp>;
-    kernel<<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, loss, (float2*)stats);
+    kernel<<<(unsigned)((rows + 7) / 8), kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, loss, stats);
     return cudaSuccess;
   }
   if (sh.parts == 8) return launch_cluster<T, 8>(rows, V, k, logits, ld, ids, wide, teacher, tau, loss, stats, s);
@@ -351,7 +351,7 @@ void launch_backward(hpspmm_ctx* ctx, int64_t rows, int V, int k, const void* lo
                  : k <= kFewEntriesWarp ? distill_backward_kernel<T, 32, kFewEntriesWarp>
                                         : distill_backward_kernel<T, 32, kMaxEntriesWarp>;
   const int64_t blocks = sh.warp ? (rows + 7) / 8 : rows * sh.parts;
-  kernel<<<(unsigned)blocks, kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, (const float2*)stats, dloss, stride,
+  kernel<<<(unsigned)blocks, kThreads, 0, s>>>(rows, V, k, (const T*)logits, ld, ids, wide, teacher, tau, stats, dloss, stride,
                                                (T*)dlogits, sh.parts);
 }
 

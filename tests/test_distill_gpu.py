@@ -453,3 +453,19 @@ def test_teachers_that_are_no_number_do_not_count(ops, V, k):
         teacher[4, :2], teacher[4, 2:4] = float("nan"), -INF
         loss, dz = _check(ops, z, ids, teacher, 1.3)
         assert loss[2] == 0 and not dz[2].any() and bool(torch.isfinite(loss).all()) and bool(torch.isfinite(dz).all())
+
+
+def test_statistics_on_any_4_bytes(ops, pkg, gpu_ctx):
+    """They are T x 2 floats and may begin where floats may."""
+    gen = torch.Generator("cuda").manual_seed(37)
+    for T, V in ((5, 300), (40, 3001), (3, 40_000)):
+        z, ids, teacher = _inputs(T, V, 7, torch.float32, gen)
+        loss, stats = torch.ops.hpspmm.topk_distill(z, ids, teacher, 1.2)
+        room = torch.full((2 * T + 3,), 7.0, device="cuda")
+        odd, loss2 = room[1:2 * T + 1], torch.empty_like(loss)
+        torch.cuda.synchronize()
+        gpu_ctx.topk_distill_forward(T, V, 7, pkg.TYPE_F32, z.data_ptr(), V, ids.data_ptr(), 8, teacher.data_ptr(), 1.2, loss2.data_ptr(), odd.data_ptr())
+        torch.cuda.synchronize()
+        assert torch.equal(odd.view(T, 2), stats) and torch.equal(loss, loss2) and bool((room[[0, -2, -1]] == 7).all())
+        dloss, back = torch.ones(T, device="cuda"), torch.ops.hpspmm.topk_distill_backward
+        assert torch.equal(back(dloss, z, ids, teacher, odd.view(T, 2), 1.2), back(dloss, z, ids, teacher, stats, 1.2))
