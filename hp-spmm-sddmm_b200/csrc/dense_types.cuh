@@ -55,6 +55,9 @@ static inline int dense_type_size(int32_t type) {
   return type == HPSPMM_TYPE_F32 ? 4 : (type == HPSPMM_TYPE_F16 || type == HPSPMM_TYPE_BF16 ? 2 : 0);
 }
 
+// Whether an array of elements of `size` bytes may begin there (a device would fault on one that may not).
+static inline bool may_begin(const void* p, int size) { return ((uintptr_t)p & (uintptr_t)(size - 1)) == 0; }
+
 // ids of 4 or 8 bytes; -1 where the id lies outside [0, n)
 __device__ __forceinline__ int load_id(const void* ids, int wide, int64_t at, int n) {
   const int64_t id = wide ? static_cast<const long long*>(ids)[at] : (int64_t) static_cast<const int*>(ids)[at];

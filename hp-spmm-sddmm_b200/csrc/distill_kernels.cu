@@ -379,6 +379,9 @@ int hpspmm_topk_distill_forward(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t k
   if (st != HPSPMM_OK) return st;
   if (T == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, loss && (V == 0 || logits) && (k == 0 || (ids && teacher_logits)), "null pointer");
+  HPSPMM_REQUIRE(ctx, may_begin(logits, dense_type_size(type)) && may_begin(loss, 4) && may_begin(stats, 4) &&
+                          (k == 0 || (may_begin(ids, id_bytes) && may_begin(teacher_logits, 4))),
+                 "an array does not begin on a multiple of its elements' size");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   const int wide = id_bytes == 8;
@@ -405,6 +408,9 @@ int hpspmm_topk_distill_backward(hpspmm_ctx* ctx, int64_t T, int64_t V, int64_t 
   HPSPMM_REQUIRE(ctx, dloss_stride >= 0, "negative stride");
   if (T == 0 || V == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, logits && stats && dloss && dlogits && (k == 0 || (ids && teacher_logits)), "null pointer");
+  HPSPMM_REQUIRE(ctx, may_begin(logits, dense_type_size(type)) && may_begin(dlogits, dense_type_size(type)) && may_begin(stats, 4) &&
+                          may_begin(dloss, 4) && (k == 0 || (may_begin(ids, id_bytes) && may_begin(teacher_logits, 4))),
+                 "an array does not begin on a multiple of its elements' size");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   const int wide = id_bytes == 8;

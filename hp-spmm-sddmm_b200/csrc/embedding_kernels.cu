@@ -595,6 +595,9 @@ int hpspmm_embedding_forward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, i
   HPSPMM_REQUIRE(ctx, ld_table >= K, "row stride below the number of columns");
   if (T == 0 || K == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, ids && out && (table || N == 0), "null pointer");
+  const int size = dense_type_size(type);
+  HPSPMM_REQUIRE(ctx, may_begin(ids, id_bytes) && may_begin(table, size) && may_begin(out, size),
+                 "an array does not begin on a multiple of its elements' size");
   // a group of lanes moves at least four elements of each of its lanes, or a row of up to 32 vectors
   if (T > ((int64_t)1 << 33) / ((K + 127) / 128)) return hpspmm_unsupported(ctx, "more than 2^31 - 1 blocks");
   hpspmm_device_guard guard(ctx->device);
@@ -623,6 +626,9 @@ int hpspmm_embedding_backward(hpspmm_ctx* ctx, int64_t T, int64_t N, int64_t K, 
   if (st != HPSPMM_OK) return st;
   if (N == 0 || K == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, dTable && (T == 0 || (ids && dOut && workspace)), "null pointer");
+  const int size = dense_type_size(type);
+  HPSPMM_REQUIRE(ctx, may_begin(dTable, size) && (T == 0 || (may_begin(ids, id_bytes) && may_begin(dOut, size))),
+                 "an array does not begin on a multiple of its elements' size");
   const backward_plan p = plan_backward(T, N, K);
   HPSPMM_REQUIRE(ctx, T == 0 || workspace_bytes >= p.bytes, "workspace too small");
   HPSPMM_REQUIRE(ctx, T == 0 || ((uintptr_t)workspace & 255) == 0, "workspace not aligned to 256 bytes");

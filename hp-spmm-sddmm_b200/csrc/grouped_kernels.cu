@@ -422,6 +422,9 @@ int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int
   HPSPMM_REQUIRE(ctx, ldx >= 0, "negative row stride");
   if (R == 0 || N == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, offsets && Y && (K == 0 || (X && (W || G == 0))), "null pointer");
+  const int size = dense_type_size(type);
+  HPSPMM_REQUIRE(ctx, may_begin(offsets, 4) && may_begin(Y, size) && may_begin(X, size) && may_begin(W, size),
+                 "an array does not begin on a multiple of its elements' size");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   if (K == 0 || G == 0) {
@@ -467,6 +470,9 @@ int hpspmm_grouped_weight_grad(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K,
   HPSPMM_REQUIRE(ctx, ldx >= 0 && ldy >= 0, "negative row stride");
   if (G == 0 || K == 0 || N == 0) return HPSPMM_OK;
   HPSPMM_REQUIRE(ctx, offsets && dW && (R == 0 || (X && dY)), "null pointer");
+  const int size = dense_type_size(type);
+  HPSPMM_REQUIRE(ctx, may_begin(offsets, 4) && may_begin(dW, size) && may_begin(X, size) && may_begin(dY, size),
+                 "an array does not begin on a multiple of its elements' size");
   hpspmm_device_guard guard(ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   if (R == 0) {

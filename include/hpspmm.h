@@ -324,10 +324,10 @@ HPSPMM_API int hpspmm_layer_update_values(hpspmm_ctx* ctx, hpspmm_layer* layer,
  * Operators next to the sparse products whose pattern is so regular that no CSR of it is built: one entry to a row
  * (rows of a table by id), one block to a group of rows (a matrix for each relation type or expert), a few samples to a
  * row (a teacher's largest logits).  Element types below; sums are kept in 32 bits and rounded once.  Rows of the
- * operands that are read may lie `ld` elements apart, what is written is contiguous.  All of them only enqueue
- * kernels: no allocation, no synchronisation, no state between calls (but hpspmm_ctx_timeouts), so they can be captured into a CUDA graph, and
- * calls that share a context may overlap on the GPU (not on the host: one call on a context at a time).  The
- * reference has no counterpart. */
+ * operands that are read may lie `ld` elements apart, what is written is contiguous; arrays begin on a multiple of their
+ * elements' size.  All of them only enqueue kernels: no allocation, no synchronisation, no state between calls (but for
+ * hpspmm_ctx_timeouts), so they can be captured into a CUDA graph, and calls that share a context may overlap on the GPU
+ * (not on the host: one call on a context at a time).  The reference has no counterpart. */
 enum { HPSPMM_TYPE_F32 = 0, HPSPMM_TYPE_F16 = 1, HPSPMM_TYPE_BF16 = 2 };
 
 /* out[t, :] = scale * table[ids[t], :]    table N x K, out T x K; ids of id_bytes (4 or 8) bytes.  An id outside

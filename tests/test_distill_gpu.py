@@ -469,3 +469,25 @@ def test_statistics_on_any_4_bytes(ops, pkg, gpu_ctx):
         assert torch.equal(odd.view(T, 2), stats) and torch.equal(loss, loss2) and bool((room[[0, -2, -1]] == 7).all())
         dloss, back = torch.ones(T, device="cuda"), torch.ops.hpspmm.topk_distill_backward
         assert torch.equal(back(dloss, z, ids, teacher, odd.view(T, 2), 1.2), back(dloss, z, ids, teacher, stats, 1.2))
+
+
+def test_arrays_off_their_elements_are_refused(pkg, gpu_ctx):
+    """Every array of every dense operator, by one byte and by half an element: the host says no before anything is launched."""
+    t = torch.zeros(4096, device="cuda")
+    a, f32, bf16 = t.data_ptr(), pkg.TYPE_F32, pkg.TYPE_BF16
+    calls = [(gpu_ctx.embedding_forward, [4, 4, 4, f32, a, 8, a, 4, 1.0, a], {4: 4, 6: 2, 9: 2}),
+             (gpu_ctx.embedding_forward, [4, 4, 4, bf16, a, 4, a, 4, 1.0, a], {4: 2, 6: 1, 9: 1}),
+             (gpu_ctx.embedding_backward, [4, 4, 4, f32, a, 8, a, 4, 1.0, a, a, 16384], {4: 4, 6: 2, 9: 2, 10: 128}),
+             (gpu_ctx.embedding_backward, [4, 4, 4, bf16, a, 4, a, 4, 1.0, a, a, 16384], {4: 2, 6: 1, 9: 1}),
+             (gpu_ctx.grouped_product, [4, 1, 4, 4, f32, a, 4, a, 0, a, a], {5: 2, 7: 2, 9: 2, 10: 2}),
+             (gpu_ctx.grouped_product, [4, 1, 4, 4, bf16, a, 4, a, 1, a, a], {5: 1, 7: 1, 9: 2, 10: 1}),
+             (gpu_ctx.grouped_weight_grad, [4, 1, 4, 4, f32, a, 4, a, 4, a, a, 0], {5: 2, 7: 2, 9: 2, 10: 2}),
+             (gpu_ctx.grouped_weight_grad, [4, 1, 4, 4, bf16, a, 4, a, 4, a, a, 1], {5: 1, 7: 1, 9: 2, 10: 1}),
+             (gpu_ctx.topk_distill_forward, [4, 4, 2, f32, a, 4, a, 8, a, 1.0, a, a], {4: 2, 6: 4, 8: 2, 10: 2, 11: 2}),
+             (gpu_ctx.topk_distill_backward, [4, 4, 2, bf16, a, 4, a, 4, a, 1.0, a, a, 1, a], {4: 1, 6: 2, 8: 2, 10: 2, 11: 2, 13: 1})]
+    for call, args, places in calls:
+        for at, off in places.items():
+            for by in {off, 1}:
+                with pytest.raises(pkg.HpspmmError) as e:
+                    call(*(args[:at] + [a + by] + args[at + 1:]))
+                assert e.value.status == pkg.ERR_INVALID
