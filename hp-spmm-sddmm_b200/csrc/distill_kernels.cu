@@ -110,7 +110,7 @@ struct running {
 
 // One pass over the row, everything in registers: NT threads to a row, CL blocks of a cluster to one where rows are few.
 // Bound by the reads of the logits; an element costs one ex2 and about five other instructions.  4,096 x 131,072 bf16: 184 us,
-// 5.8 TB/s; 1,021 x 32,003 floats: 32 us, 4.0 TB/s; 8 rows of 131,072 f16 in clusters of eight: 5.0 us.
+// 5.8 TB/s; 1,021 x 32,003 floats: 32 us, 4.0 TB/s; 8 rows of 131,072 f16 in clusters of eight: 5.2 us.
 template <typename T, int NT, int CL, int ENTRIES>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 0)
 distill_forward_kernel(int64_t rows, int V, int k, const T* __restrict__ logits, int64_t ld, const void* __restrict__ ids, int wide,

@@ -9,9 +9,11 @@
 // 256: a tile costs as much as the rows that its group has, whether that is one row or 256, and a lane's neighbours hold
 // neighbouring columns of Y, so that a warp's stores are contiguous.  Blocks stay for the whole call (one to an SM) and take
 // tiles in turn; the tiles follow from the offsets, which only the device knows.  Bound by the tensor cores and, in a row of
-// such calls, by the power they take: 32,768 rows of 8 groups, 2048 x 5632, bf16, alone 1.29 to 1.44 PFLOP/s; a step of a
-// decoder (56 rows in 64 groups, 2048 x 1536) by the bytes of the matrices: 6.2 TB/s.
-// Large calls take tiles of 256 x 256 in pairs of blocks (cta_group::2).  Where the tiles are fewer than the SMs (a step of a decoder), clusters of 2 to 8 blocks split the depth of one tile and
+// such calls, by the power they take: 32,768 rows of 8 groups, 2048 x 5632, bf16, alone 1.29 to 1.44 PFLOP/s; 16,384 rows of 32
+// groups, 2048 x 2816, 1.1 alone and 0.9 in a row; a step of a decoder (56 rows in 64 groups, 2048 x 1536) by the bytes of the
+// matrices: 6.2 TB/s.
+// Large calls take tiles of 256 x 256 in pairs of blocks (cta_group::2).  Where the tiles are fewer than the SMs (a step of a
+// decoder), clusters of 2 to 8 blocks split the depth of one tile and
 // add their parts through distributed shared memory, in the order of their ranks.
 #include <cuda.h>
 

@@ -349,9 +349,9 @@ HPSPMM_API int hpspmm_embedding_backward(hpspmm_ctx* ctx, int64_t T, int64_t N, 
 /* Y[r, :] = X[r, :] * W[g] for the rows offsets[g] <= r < offsets[g + 1] of group g: X R x K, Y R x N, W G matrices
  * K x N one after the other (w_out_first = 0) or stored transposed, N x K (w_out_first = 1), offsets G + 1 ascending
  * device ints in [0, R].  Rows in front of the first group and behind the last one become zeros.  The gradient of X is
- * the same call with dY, K and N exchanged and the other w_out_first.  Offsets that do not ascend give rows of no use,
- * but nothing outside the operands is read or written.  R, K and N are at most 2^31 - 1026, K at most 2^27 for the 16-bit
- * types, G at most 2^20. */
+ * the same call with dY, K and N exchanged and the other w_out_first.  Offsets that do not ascend give rows of no use
+ * and take as long as all the rows that they name, but nothing outside the operands is read or written.  R, K and N are at
+ * most 2^31 - 1026, K at most 2^27 for the 16-bit types, G at most 2^20. */
 HPSPMM_API int hpspmm_grouped_product(hpspmm_ctx* ctx, int64_t R, int64_t G, int64_t K, int64_t N,
                                       int32_t type, const void* X, int64_t ldx, const void* W,
                                       int32_t w_out_first, const int32_t* offsets, void* Y,
