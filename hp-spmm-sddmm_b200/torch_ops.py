@@ -195,5 +195,7 @@ def timeouts(device=None):
     """How many blocks of the grouped products' tensor-core kernels have given up a wait on this GPU (expected 0; what
     such a call wrote is not to be used).  Waits for the device.  The first call of these operators that finds such a product
     done raises an error by itself; after a last step, or replays of a graph, ask here."""
-    index = None if device is None else torch.device(device).index
-    return _C.timeouts(torch.cuda.current_device() if index is None else index)
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise RuntimeError("hpspmm: waits are counted on a CUDA device, got %s" % device)
+    return _C.timeouts(torch.cuda.current_device() if device.index is None else device.index)

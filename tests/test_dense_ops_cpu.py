@@ -75,3 +75,9 @@ def test_sizes_whose_last_tile_would_pass_2_31(pkg):
             assert need(most, 1, 8, 8, type, out_first) > 0 and need(5, 1, most, 8, type, out_first) == 0
             for sizes in ((most + 1, 1, 8, 8), (2 ** 31 - 2, 1, 8, 8), (5, 1, most + 1, 8), (5, 1, 8, most + 1), (5, 2 ** 20 + 1, 8, 8)):
                 assert need(*sizes, type, out_first) == -1
+
+
+def test_waits_are_asked_for_on_a_gpu(pkg):
+    for device in ("cpu", torch.device("meta")):
+        with pytest.raises(RuntimeError, match="hpspmm: waits are counted on a CUDA device"):
+            ref.ops_of(pkg).timeouts(device)
